@@ -14,7 +14,10 @@ LIB = os.path.join(LIBDIR, "libhumanvid_hip.so")
 UNITS = ["hv_api.cpp", "k_gemm.hip", "k_conv.hip", "k_norm.hip", "k_attention.hip", "k_temporal.hip",
          "k_elementwise.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-I" + os.path.join(REPO, "include"), "-I" + CSRC]
+# packed fp32 instructions (v_pk_add / mul / fma_f32), which -O3 forms from ordinary float code, are switched off: some of their
+# forms have given wrong results on this hardware (hipcc's host pass does not know the feature and warns: harmless)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+         "-I" + os.path.join(REPO, "include"), "-I" + CSRC]
 
 
 def _newer(target, deps):
