@@ -92,7 +92,27 @@ class TemporalAttentionParams(_S):
     ]
 
 
-_STRUCTS = (GemmParams, Conv3x3Params, GroupNormParams, AttentionParams, TemporalAttentionParams, GnPartsParams)
+class CrossAttentionParams(C.Structure):  # filled by position (ops.cross_attention): a latency-bound call at small sizes
+    _fields_ = [
+        ("Q", P), ("ldq", L), ("q_stride_b", L), ("K", P), ("ldk", L), ("k_stride_b", L), ("V", P), ("ldv", L),
+        ("v_stride_b", L), ("O", P), ("ldo", L), ("o_stride_b", L),
+        ("kv_len", P), ("key_mask", P), ("mask_stride_b", L),
+        ("B", I), ("Lq", I), ("Lk", I), ("heads", I), ("kv_heads", I), ("D", I), ("scale", F),
+        ("workspace", P), ("workspace_floats", L),
+    ]
+
+
+class GemmFp8Params(C.Structure):  # filled by position (ops.gemm_fp8)
+    _fields_ = [
+        ("X", P), ("ldx", L), ("x_scale", P), ("x_scale_row", L), ("x_scale_k", L),
+        ("W", P), ("ldw", L), ("w_scale", P), ("w_scale_row", L), ("w_scale_k", L),
+        ("Y", P), ("ldy", L), ("out_f32", I), ("M", I), ("N", I), ("K", I),
+        ("bias", P), ("residual", P), ("ldr", L), ("workspace", P), ("workspace_floats", L),
+    ]
+
+
+_STRUCTS = (GemmParams, Conv3x3Params, GroupNormParams, AttentionParams, TemporalAttentionParams, GnPartsParams,
+            CrossAttentionParams, GemmFp8Params)
 
 # every symbol include/humanvid_hip.h declares: name -> (restype, argtypes)
 PROTOTYPES = {
@@ -111,6 +131,11 @@ PROTOTYPES = {
     "hv_attention": (I, [C.POINTER(AttentionParams), P]),
     "hv_attention_fp8_quantize": (I, [P, L, P, L, I, I, I, I, P, P, P, P, L, P, L, I, P]),
     "hv_attention_fp8": (I, [C.POINTER(AttentionParams), P, P, P, P, P]),
+    "hv_cross_attention": (I, [C.POINTER(CrossAttentionParams), P]),
+    "hv_cross_attention_workspace": (L, [C.POINTER(CrossAttentionParams)]),
+    "hv_fp8_quantize": (I, [P, L, I, I, I, P, L, P, L, L, P]),
+    "hv_gemm_fp8": (I, [C.POINTER(GemmFp8Params), P]),
+    "hv_gemm_fp8_workspace": (L, [C.POINTER(GemmFp8Params)]),
     "hv_set_tuning": (I, [I, I]),
     "hv_temporal_attention": (I, [C.POINTER(TemporalAttentionParams), P]),
     "hv_pack_ncfhw": (I, [P, I, I, I, I, I, I, P, I, I, P, I, P]),

@@ -12,7 +12,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libhumanvid_hip.so")
 UNITS = ["hv_api.cpp", "k_gemm.hip", "k_conv.hip", "k_norm.hip", "k_attention.hip", "k_temporal.hip",
-         "k_elementwise.hip"]
+         "k_elementwise.hip", "k_cross.hip", "k_fp8.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # packed fp32 instructions (v_pk_add / mul / fma_f32), which -O3 forms from ordinary float code, are switched off: some of their
 # forms have given wrong results on this hardware (hipcc's host pass does not know the feature and warns: harmless)

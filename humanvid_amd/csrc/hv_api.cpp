@@ -38,7 +38,8 @@ int hv_abi_version(void) { return 2; }  // 2: gn_part fields, hv_groupnorm_from_
 int hv_struct_sizes(int* out, int capacity) {
     const int s[] = {(int)sizeof(hv_gemm_params),      (int)sizeof(hv_conv3x3_params),
                      (int)sizeof(hv_groupnorm_params), (int)sizeof(hv_attention_params),
-                     (int)sizeof(hv_temporal_attention_params), (int)sizeof(hv_gn_parts_params)};
+                     (int)sizeof(hv_temporal_attention_params), (int)sizeof(hv_gn_parts_params),
+                     (int)sizeof(hv_cross_attention_params), (int)sizeof(hv_gemm_fp8_params)};
     const int n = (int)(sizeof(s) / sizeof(s[0]));
     for (int i = 0; i < n && i < capacity; ++i) out[i] = s[i];
     return n;
@@ -121,6 +122,48 @@ int hv_attention_fp8(const hv_attention_params* p, const float* kscale, const fl
     return hv_check_launch("hv_attention_fp8");
 }
 
+int hv_cross_attention(const hv_cross_attention_params* p, void* stream) {
+    if (!p) return hv_fail(HV_EINVAL, "hv_cross_attention: null parameters");
+    if (p->B > 0 && p->Lq > 0 && (!p->Q || !p->O || (p->Lk > 0 && (!p->K || !p->V)))) return hv_fail(HV_EINVAL, "hv_cross_attention: null operand");
+    int rc = hvk_cross_attention(*p, (hipStream_t)stream);
+    if (rc == -2) return hv_fail(HV_ENOTSUP, "hv_cross_attention: head dim must be 40, 64, 80, 128 or 160");
+    if (rc == -3) return hv_fail(HV_EINVAL, "hv_cross_attention: workspace smaller than hv_cross_attention_workspace() floats");
+    if (rc != 0)
+        return hv_fail(HV_EINVAL, "hv_cross_attention: need sizes >= 0, heads a multiple of kv_heads, a positive finite scale, 16-byte aligned "
+                                  "pointers and strides (multiples of 8 elements)");
+    return hv_check_launch("hv_cross_attention");
+}
+long hv_cross_attention_workspace(const hv_cross_attention_params* p) {
+    if (!p) return hv_fail(HV_EINVAL, "hv_cross_attention_workspace: null parameters");
+    const long n = hvk_cross_attention_workspace(*p);
+    if (n == -2) return hv_fail(HV_ENOTSUP, "hv_cross_attention_workspace: head dim must be 40, 64, 80, 128 or 160");
+    if (n < 0) return hv_fail(HV_EINVAL, "hv_cross_attention_workspace: need sizes >= 0 and heads a multiple of kv_heads");
+    return n;
+}
+
+int hv_fp8_quantize(const uint16_t* X, long ldx, int M, int K, int block_rows, uint8_t* Q, long ldq, float* scale, long scale_row,
+                    long scale_k, void* stream) {
+    if (M > 0 && (!X || !Q || !scale)) return hv_fail(HV_EINVAL, "hv_fp8_quantize: null operand");
+    if (hvk_fp8_quantize(X, ldx, M, K, block_rows, Q, ldq, scale, scale_row, scale_k, (hipStream_t)stream) != 0)
+        return hv_fail(HV_EINVAL, "hv_fp8_quantize: need M >= 0, K a positive multiple of 16, block_rows 1 or 128, 16-byte aligned rows");
+    return hv_check_launch("hv_fp8_quantize");
+}
+
+int hv_gemm_fp8(const hv_gemm_fp8_params* p, void* stream) {
+    if (!p) return hv_fail(HV_EINVAL, "hv_gemm_fp8: null parameters");
+    if (p->M > 0 && p->N > 0 && (!p->X || !p->W || !p->Y || !p->x_scale || !p->w_scale)) return hv_fail(HV_EINVAL, "hv_gemm_fp8: null operand");
+    const int rc = hvk_gemm_fp8(*p, (hipStream_t)stream);
+    if (rc == -3) return hv_fail(HV_EINVAL, "hv_gemm_fp8: workspace smaller than hv_gemm_fp8_workspace() floats");
+    if (rc != 0) return hv_fail(HV_EINVAL, "hv_gemm_fp8: need M, N >= 0, K a positive multiple of 16, X and W rows 16-byte aligned with strides up to 8 MiB");
+    return hv_check_launch("hv_gemm_fp8");
+}
+long hv_gemm_fp8_workspace(const hv_gemm_fp8_params* p) {
+    if (!p) return hv_fail(HV_EINVAL, "hv_gemm_fp8_workspace: null parameters");
+    const long n = hvk_gemm_fp8_workspace(*p);
+    if (n < 0) return hv_fail(HV_EINVAL, "hv_gemm_fp8_workspace: need M, N >= 0 and K a positive multiple of 16");
+    return n;
+}
+
 static int g_hv_cmdlist_fallbacks = 0;  // command lists whose graph capture failed (hv_cmdlist_fallbacks())
 static int g_hv_cmdlist_graphs = 1;  // hv_set_tuning(HV_TUNE_CMDLIST_GRAPHS): 0 = hv_cmdlist_run re-issues the closures on every run (A/B)
 int hv_set_tuning(int key, int value) {
@@ -135,6 +178,7 @@ int hv_set_tuning(int key, int value) {
     else if (key == HV_TUNE_CONV_BIG && (value >= 0 && value <= 3)) hvk_conv_use_big(value);
     else if (key == HV_TUNE_CONV_RASTER && (value >= 0 && value <= 2)) hvk_conv_raster(value);
     else if (key == HV_TUNE_CONV_W4 && (value >= 0 && value <= 3)) hvk_conv_use_w4(value);
+    else if (key == HV_TUNE_GEMM_FP8 && (value == 0 || value == 64 || value == 128 || value == 256)) hvk_gemm_fp8_tile(value);
     else if (key == HV_TUNE_CMDLIST_GRAPHS && (value == 0 || value == 1)) g_hv_cmdlist_graphs = value;
     else return hv_fail(HV_EINVAL, "hv_set_tuning: unknown key/value");
     return HV_OK;

@@ -1,0 +1,358 @@
+// hv_cross_attention.h -- attention of Lq queries to an encoder's Lk states (Lk of any length, unrelated to Lq), with a key
+// mask, attended lengths and shared key heads.  The UNets' attn2 with more than one encoder token
+// (/root/reference/src/models/attention.py:410-424, diffusers Attention with encoder_hidden_states).
+//
+//   s[i][j] = scale * q[i] . k[j],  p = softmax over the attended j,  o[i] = sum_j p[i][j] v[j]      (0 where nothing is attended)
+//
+// One pass over the states with the running maximum m and sum l of the softmax: a chunk of CH = 32 NP keys contributes
+//   m' = max(m, max_j s),  p_j = 2^((s_j - m') scale log2 e),  (l, o) = (l, o) 2^((m - m') scale log2 e) + sum_j p_j (1, v_j).
+// m, l and o are fp32; p is rounded to bf16 for the second product (2^-8 relative, the operands' own precision), and l sums
+// those rounded p (a product with a row of ones), so that the weights of a row add up to one exactly.
+//
+// Layout: S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16.  A lane owns one query column (lane & 15) and 4 of every 16
+// key rows ((lane >> 4) * 4 + r): the maximum needs two lane-swap steps per chunk, and the p of two 16-key tiles ARE the B
+// operand of the second product if its reduction index runs over the keys in that order (k = 8 g + e is key 4 g + e of the
+// first tile for e < 4, of the second for e >= 4); V is stored row-major in LDS and read transposed in the same order.
+// A masked key's row of K and V is zero in LDS (whatever memory holds there) and its score starts at -inf: the accumulator of
+// the first product is initialised with the chunk's bias (0 / -inf) instead of zero, so masks cost no instruction.
+// Query heads that share a key head are rows of the same tile: row r of a (batch, key head) is query r / G, head r % G.
+#pragma once
+#include "hv_common.h"
+#include "humanvid_hip.h"
+
+#ifndef HV_EMU
+// max over the four lanes with equal lane & 15
+HV_DEV float hv_max_quarters(float x) {
+    // (the halves are copied out first: a bit cast of a vector element takes element 0)
+    unsigned u = __builtin_bit_cast(unsigned, x);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // a[0]: the lower half's values in both halves, a[1]: the upper's
+    unsigned lo = a[0], hi = a[1];
+    x = fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+    u = __builtin_bit_cast(unsigned, x);
+    const auto b = __builtin_amdgcn_permlane16_swap(u, u, false, false);  // the same for the two 16-lane rows of a half
+    lo = b[0], hi = b[1];
+    return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+}
+#else
+HV_DEV float hv_max_quarters(float x) {
+    x = fmaxf(x, __shfl_xor(x, 32));
+    return fmaxf(x, __shfl_xor(x, 16));
+}
+#endif
+
+struct HvCrossArgs {
+    hv_cross_attention_params p;
+    int G, rows;         // heads per key head; Lq * G
+    int blocks, per_wg;  // row blocks of a (batch, key head); consecutive blocks one workgroup takes
+    int groups;          // ceil(blocks / per_wg)
+    int units;           // workgroups with work
+    int splits;          // ranges the keys are cut into
+    float c;             // scale * log2 e
+};
+
+template <int D, int QT, int NP>
+__global__ __launch_bounds__(256) void hv_cross_attention_kernel(HvCrossArgs a) {
+    constexpr int KS = (D + 31) / 32, DT = (D + 15) / 16, P8 = D / 8, CH = 32 * NP;
+    constexpr int KSTR = KS * 64 + 16;                     // bytes of a K row: an odd number of 16-byte pieces (no bank conflicts)
+    constexpr int VSTR = (DT % 2 ? DT : DT + 1) * 32;      // bytes of a V row: an odd number of 32-byte tiles (the transposed reads)
+    constexpr int NV = (CH * P8 + 255) / 256;              // 16-byte pieces of K (and of V) that a thread stages
+    __shared__ __attribute__((aligned(16))) unsigned char sK[CH * KSTR];
+    __shared__ __attribute__((aligned(16))) unsigned char sV[CH * VSTR];
+    __shared__ __attribute__((aligned(16))) float sBias[CH];
+
+    // neighbouring units (the heads of one row block, then the next row blocks) run on one XCD: their query rows share cache lines
+    const int per_xcd = (a.units + 7) / 8;
+    const int unit = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per_xcd || unit >= a.units) return;
+    const hv_cross_attention_params& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+    const int kvh = unit % p.kv_heads;
+    int rest = unit / p.kv_heads;
+    const int split = rest % a.splits;
+    rest /= a.splits;
+    const int group = rest % a.groups, b = rest / a.groups;
+
+    int len = p.kv_len ? p.kv_len[b] : p.Lk;
+    len = len < 0 ? 0 : len > p.Lk ? p.Lk : len;
+    int k_begin = 0, k_end = len;
+    if (a.splits > 1) {
+        const int per = ((len + a.splits - 1) / a.splits + 31) / 32 * 32;
+        k_begin = min(split * per, len);
+        k_end = min(k_begin + per, len);
+    }
+    const int chunks = (k_end - k_begin + CH - 1) / CH;
+    const bf16_t* Kb = p.K + (long)b * p.k_stride_b + (long)kvh * D;
+    const bf16_t* Vb = p.V + (long)b * p.v_stride_b + (long)kvh * D;
+    const uint8_t* mask = p.key_mask ? p.key_mask + (long)b * p.mask_stride_b : nullptr;
+
+    // the zero columns D .. 32 KS of K and D .. 16 DT of V: written once, staging leaves them alone
+    const u32x4 zero4 = {0u, 0u, 0u, 0u};
+    if constexpr (KS * 4 > P8) {
+        for (int i = tid; i < CH * (KS * 4 - P8); i += 256)
+            hv_st16(sK + (i / (KS * 4 - P8)) * KSTR + (P8 + i % (KS * 4 - P8)) * 16, zero4);
+    }
+    if constexpr (DT * 2 > P8) {
+        for (int i = tid; i < CH; i += 256) hv_st16(sV + i * VSTR + P8 * 16, zero4);
+    }
+
+    u32x4 kreg[NV], vreg[NV];
+    float breg = 0.f;
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = tid + i * 256, row = k0 + idx / P8, piece = idx % P8;
+            const bool on = idx < CH * P8 && row < k_end && (mask == nullptr || mask[row] != 0);
+            kreg[i] = on ? hv_ld16(Kb + (long)row * p.ldk + piece * 8) : zero4;
+            vreg[i] = on ? hv_ld16(Vb + (long)row * p.ldv + piece * 8) : zero4;
+        }
+        if (tid < CH) {
+            const int row = k0 + tid;
+            breg = row < k_end && (mask == nullptr || mask[row] != 0) ? 0.f : -INFINITY;
+        }
+    };
+    auto stage = [&]() {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = tid + i * 256;
+            if (idx < CH * P8) {
+                hv_st16(sK + (idx / P8) * KSTR + (idx % P8) * 16, kreg[i]);
+                hv_st16(sV + (idx / P8) * VSTR + (idx % P8) * 16, vreg[i]);
+            }
+        }
+        if (tid < CH) sBias[tid] = breg;
+    };
+    if (chunks == 1) {  // the states fit one chunk: they stay in LDS for all row blocks
+        fetch(k_begin);
+        stage();
+        __syncthreads();
+    }
+
+    const int blk_end = min((group + 1) * a.per_wg, a.blocks);
+    for (int blk = group * a.per_wg; blk < blk_end; ++blk) {
+        const int r0 = (blk * 4 + wave) * QT * 16 + col;
+        bf16x8 qf[QT][KS];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int r = r0 + t * 16;
+            const bf16_t* src = p.Q + (long)b * p.q_stride_b + (long)(r / a.G) * p.ldq + (long)(kvh * a.G + r % a.G) * D;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                qf[t][ks] = hv_as_bf16x8(r < a.rows && ks * 32 + g * 8 < D ? hv_ld16(src + ks * 32 + g * 8) : zero4);
+        }
+        f32x4 acc[QT][DT], lsum[QT];
+        float m[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            m[t] = -INFINITY;
+            lsum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        if (chunks > 1) fetch(k_begin);
+        for (int ch = 0; ch < chunks; ++ch) {
+            const int n = k_end - k_begin - ch * CH;  // keys left
+            if (chunks > 1) {
+                __syncthreads();  // the readers of the previous chunk are done
+                stage();
+                __syncthreads();
+                if (ch + 1 < chunks) fetch(k_begin + (ch + 1) * CH);
+            }
+            f32x4 s[QT][2 * NP];
+            float top[QT];
+#pragma unroll
+            for (int t = 0; t < QT; ++t) top[t] = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < 2 * NP; ++kt) {
+                if ((kt & ~1) * 16 < n) {
+                    const f32x4 bias = *reinterpret_cast<const f32x4*>(sBias + kt * 16 + g * 4);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) s[t][kt] = bias;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        const bf16x8 kf = hv_as_bf16x8(hv_ld16(sK + (kt * 16 + col) * KSTR + ks * 64 + g * 16));
+#pragma unroll
+                        for (int t = 0; t < QT; ++t) s[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][ks], s[t][kt], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int t = 0; t < QT; ++t)
+                        top[t] = fmaxf(fmaxf(top[t], fmaxf(s[t][kt][0], s[t][kt][1])), fmaxf(s[t][kt][2], s[t][kt][3]));
+                }
+            }
+            float mc[QT];
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                const float mn = fmaxf(m[t], hv_max_quarters(top[t]));
+                const float ms = mn == -INFINITY ? 0.f : mn;  // nothing attended yet: 2^(-inf - 0) = 0, not 2^(-inf + inf)
+                const float alpha = __builtin_amdgcn_exp2f((m[t] - ms) * a.c);
+                m[t] = mn;
+                mc[t] = -ms * a.c;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) lsum[t][e] *= alpha;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[t][d][e] *= alpha;
+            }
+#pragma unroll
+            for (int pr = 0; pr < NP; ++pr) {
+                if (pr * 32 < n) {
+                    bf16x8 pf[QT];
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) {
+                        float f[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) f[e] = __builtin_amdgcn_exp2f(fmaf(s[t][2 * pr + e / 4][e % 4], a.c, mc[t]));
+                        pf[t] = hv_as_bf16x8(hv_pack8(f));
+                    }
+                    const bf16x8 ones = {0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80};
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) lsum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[t], lsum[t], 0, 0, 0);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        // lane t of a 16-lane group points at row t / 4, columns 4 (t % 4) and receives column t of the 4 rows
+                        const unsigned char* src = sV + (pr * 32 + g * 4 + col / 4) * VSTR + d * 32 + (col & 3) * 8;
+                        const bf16x4 v0 = hv_lds_tr4(src), v1 = hv_lds_tr4(src + 16 * VSTR);
+                        const bf16x8 vf = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+#pragma unroll
+                        for (int t = 0; t < QT; ++t) acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], acc[t][d], 0, 0, 0);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int r = r0 + t * 16;
+            if (r >= a.rows) continue;
+            if (a.splits > 1) {  // unnormalised sums, with the maximum and the sum of weights they refer to
+                float* dst = p.workspace + ((((long)b * p.kv_heads + kvh) * a.rows + r) * a.splits + split) * (D + 2);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    if (d * 16 + g * 4 < D) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) dst[2 + d * 16 + g * 4 + e] = acc[t][d][e];
+                    }
+                if (g == 0) {
+                    dst[0] = m[t];
+                    dst[1] = lsum[t][0];
+                }
+            } else {
+                const float inv = lsum[t][0] == 0.f ? 0.f : 1.0f / lsum[t][0];
+                bf16_t* dst = p.O + (long)b * p.o_stride_b + (long)(r / a.G) * p.ldo + (long)(kvh * a.G + r % a.G) * D;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    if (d * 16 + g * 4 < D) {
+                        const u32x2 w = {hv_pack2(acc[t][d][0] * inv, acc[t][d][1] * inv), hv_pack2(acc[t][d][2] * inv, acc[t][d][3] * inv)};
+                        hv_st8(dst + d * 16 + g * 4, w);
+                    }
+            }
+        }
+    }
+}
+
+// joins the splits of a row: o = sum_s o_s 2^((m_s - m) c) / sum_s l_s 2^((m_s - m) c); one wavefront per row
+template <int D>
+__global__ __launch_bounds__(256) void hv_cross_attention_join_kernel(HvCrossArgs a) {
+    const hv_cross_attention_params& p = a.p;
+    const int lane = threadIdx.x & 63;
+    const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= (long)p.B * p.kv_heads * a.rows) return;
+    const int r = (int)(item % a.rows);
+    const int kvh = (int)(item / a.rows % p.kv_heads), b = (int)(item / a.rows / p.kv_heads);
+    const float* src = p.workspace + item * a.splits * (D + 2);
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, src[s * (D + 2)]);
+    const float ms = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[(D + 63) / 64];
+#pragma unroll
+    for (int i = 0; i < (D + 63) / 64; ++i) o[i] = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float* q = src + s * (D + 2);
+        const float w = __builtin_amdgcn_exp2f((q[0] - ms) * a.c);
+        l += w * q[1];
+#pragma unroll
+        for (int i = 0; i < (D + 63) / 64; ++i)
+            if (i * 64 + lane < D) o[i] += w * q[2 + i * 64 + lane];
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    bf16_t* dst = p.O + (long)b * p.o_stride_b + (long)(r / a.G) * p.ldo + (long)(kvh * a.G + r % a.G) * D;
+#pragma unroll
+    for (int i = 0; i < (D + 63) / 64; ++i)
+        if (i * 64 + lane < D) dst[i * 64 + lane] = hv_f2bf(o[i] * inv);
+}
+
+// sizes -> how the work is cut (also what hv_cross_attention_workspace answers from): -1 invalid, -2 head dim
+static inline int hv_cross_attention_plan(const hv_cross_attention_params& p, HvCrossArgs& a, int& qt, int& np) {
+    if (p.B < 0 || p.Lq < 0 || p.Lk < 0 || p.heads <= 0 || p.kv_heads <= 0 || p.heads % p.kv_heads != 0) return -1;
+    if (p.D != 40 && p.D != 64 && p.D != 80 && p.D != 128 && p.D != 160) return -2;
+    const long rows = (long)p.Lq * (p.heads / p.kv_heads);
+    if (rows > 0x3fffffffL) return -1;
+    a.p = p;
+    a.G = p.heads / p.kv_heads;
+    a.rows = (int)rows;
+    qt = rows > 64 ? 2 : 1;
+    np = p.Lk > 64 && p.Lk <= 96 ? 3 : 2;
+    a.blocks = (int)((rows + 64 * qt - 1) / (64 * qt));
+    const long base = (long)p.B * p.kv_heads * a.blocks;
+    a.splits = 1;
+    if (base < 512 && p.Lk >= 256) {  // too few workgroups to fill the chip: cut the keys
+        const long want = (1024 + base - 1) / (base > 0 ? base : 1), most = p.Lk / 128;
+        a.splits = (int)(want < most ? want : most);
+        if (a.splits < 1) a.splits = 1;
+    }
+    a.per_wg = 1;
+    if (p.Lk <= 32 * np) a.per_wg = (int)(base / 4096 < 1 ? 1 : base / 4096 > 16 ? 16 : base / 4096);
+    a.groups = (a.blocks + a.per_wg - 1) / a.per_wg;
+    const long units = (long)p.B * p.kv_heads * a.groups * a.splits;
+    if (units > 0x3fffffffL) return -1;
+    a.units = (int)units;
+    a.c = p.scale * 1.44269504088896341f;
+    return 0;
+}
+
+static inline long hv_cross_attention_floats(const HvCrossArgs& a) {
+    return a.splits > 1 ? (long)a.p.B * a.p.kv_heads * a.rows * a.splits * (a.p.D + 2) : 0;
+}
+
+template <int D>
+static inline void hv_cross_attention_launch_d(const HvCrossArgs& a, int qt, int np, hipStream_t stream) {
+    const dim3 grid((unsigned)((a.units + 7) / 8 * 8)), block(256);
+    hv_note("hv_cross_attention_kernel<%d,%d,%d> | B=%d Lq=%d Lk=%d heads=%d/%d splits=%d", D, qt, np, a.p.B, a.p.Lq, a.p.Lk, a.p.heads,
+            a.p.kv_heads, a.splits);
+    if (qt == 2 && np == 3) hv_launch(hv_cross_attention_kernel<D, 2, 3>, grid, block, stream, a);
+    else if (qt == 2) hv_launch(hv_cross_attention_kernel<D, 2, 2>, grid, block, stream, a);
+    else if (np == 3) hv_launch(hv_cross_attention_kernel<D, 1, 3>, grid, block, stream, a);
+    else hv_launch(hv_cross_attention_kernel<D, 1, 2>, grid, block, stream, a);
+    if (a.splits > 1) {
+        const long items = (long)a.p.B * a.p.kv_heads * a.rows;
+        hv_note("hv_cross_attention_join_kernel<%d> | rows=%ld splits=%d", D, items, a.splits);
+        hv_launch(hv_cross_attention_join_kernel<D>, dim3((unsigned)((items + 3) / 4)), block, stream, a);
+    }
+}
+
+static inline long hv_cross_attention_workspace_of(const hv_cross_attention_params& p) {
+    HvCrossArgs a;
+    int qt, np;
+    const int rc = hv_cross_attention_plan(p, a, qt, np);
+    return rc ? rc : hv_cross_attention_floats(a);
+}
+
+static inline int hv_cross_attention_launch(const hv_cross_attention_params& p, hipStream_t stream) {
+    HvCrossArgs a;
+    int qt, np;
+    const int rc = hv_cross_attention_plan(p, a, qt, np);
+    if (rc) return rc;
+    if (!(p.scale > 0.f) || p.scale > 3.0e38f) return -1;
+    if (p.B == 0 || p.Lq == 0) return 0;
+    const uint64_t addr = (uint64_t)p.Q | (uint64_t)p.K | (uint64_t)p.V | (uint64_t)p.O;
+    const long strides = p.ldq | p.ldk | p.ldv | p.ldo | p.q_stride_b | p.k_stride_b | p.v_stride_b | p.o_stride_b;
+    if ((addr & 15) != 0 || (strides & 7) != 0) return -1;
+    if (hv_cross_attention_floats(a) > p.workspace_floats || (a.splits > 1 && (p.workspace == nullptr || ((uint64_t)p.workspace & 3) != 0))) return -3;
+    switch (p.D) {
+        case 40: hv_cross_attention_launch_d<40>(a, qt, np, stream); break;
+        case 64: hv_cross_attention_launch_d<64>(a, qt, np, stream); break;
+        case 80: hv_cross_attention_launch_d<80>(a, qt, np, stream); break;
+        case 128: hv_cross_attention_launch_d<128>(a, qt, np, stream); break;
+        default: hv_cross_attention_launch_d<160>(a, qt, np, stream); break;
+    }
+    return 0;
+}

@@ -1,0 +1,495 @@
+// hv_gemm_fp8.h -- Y = X8 . W8^T in OCP e4m3 with a scale for each block of 128 of the reduction, and the quantisation that
+// makes the operands.
+//
+//   y[m][n] = bias[n] + residual[m][n] + sum_kb xs[m][kb] ws[n / 128][kb] sum_{k in block kb} x8[m][k] w8[n][k]
+//
+// A block of 128 is exactly one v_mfma_f32_16x16x128_f8f6f4: every instruction starts from a zero accumulator and its four
+// results per lane are added to the fp32 sums with the block's factor xs ws -- 4 v_fma per 32-cycle MFMA, which fit under it.
+// The operands are taken as A = W (rows n), B = X (columns m): a lane then owns ONE row m of Y per 16-row tile, so xs is one
+// value per lane and tile, and the four W tiles of a 64-column block are read from LDS in an order that leaves the lane 16
+// consecutive columns (n = 16 (lane >> 4) + 4 t + r): 16-byte stores, whole 128-byte lines per wave.
+// Both operands are read with the same lane -> k assignment, so its order inside a block does not matter to the sum.
+//
+// Precision: the 8-bit matrix instructions (16x16x128 and 16x16x32 alike) add the products of 8 neighbouring k after aligning them
+// to the largest of the eight with 13 bits kept behind it; the sums of those groups are exact to fp32 (measured, one product
+// against another).  That is 1.6e-5 of the result (2-norm) for operands of like size, 5e-5 for operands over the whole e4m3 range:
+// nothing to a bf16 output (1.7e-3), but an fp32 output would show it.  fp32 outputs are therefore computed on the bf16 instruction
+// from the operands converted in registers (every e4m3 value is a bf16 value; its sums are exact to fp32: 8e-8 measured), at twice
+// the matrix time.
+#pragma once
+#include "hv_common.h"
+#include "humanvid_hip.h"
+
+typedef int hv_i32x8 __attribute__((ext_vector_type(8)));  // 32 e4m3 values: the A / B operand of the 128-deep MFMA
+
+HV_DEV f32x4 hv_mfma_fp8_128(hv_i32x8 a, hv_i32x8 b) {  // 16 x 16 x 128 from a zero accumulator
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#ifndef HV_EMU
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, zero, 0, 0, 0, 0, 0, 0);  // e4m3 x e4m3, no hardware scale
+#else
+    return hvemu::mfma_fp8_128(a, b, zero);
+#endif
+}
+// four floats -> four e4m3 (nearest, ties to even)
+HV_DEV unsigned hv_e4m3x4(const float* f) {
+#ifndef HV_EMU
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], lo, true);
+#else
+    return hvemu::cvt_pk_fp8(f[2], f[3], hvemu::cvt_pk_fp8(f[0], f[1], 0, false), true);
+#endif
+}
+// 16 e4m3 values -> bf16, exactly
+HV_DEV void hv_e4m3_to_bf16(u32x4 v, bf16x8* out) {
+    u32x4 w[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#ifndef HV_EMU
+        const unsigned lo = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], 1.0f, false));
+        const unsigned hi = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], 1.0f, true));
+#else
+        auto two = [](unsigned b) { return hv_pack2(hvemu::fp8_to_f((unsigned char)b), hvemu::fp8_to_f((unsigned char)(b >> 8))); };
+        const unsigned lo = two(v[i]), hi = two(v[i] >> 16);
+#endif
+        w[i / 2][2 * (i % 2)] = lo;
+        w[i / 2][2 * (i % 2) + 1] = hi;
+    }
+    out[0] = hv_as_bf16x8(w[0]);
+    out[1] = hv_as_bf16x8(w[1]);
+}
+
+// a lane's 32 values of one row and block, ready for the matrix instruction: as they are, or converted (WIDE: fp32 outputs)
+template <bool WIDE>
+struct HvFp8Frag {
+    hv_i32x8 v;
+    HV_DEV void set(u32x4 lo, u32x4 hi);
+};
+template <>
+struct HvFp8Frag<true> {
+    bf16x8 v[4];
+    HV_DEV void set(u32x4 lo, u32x4 hi) {
+        hv_e4m3_to_bf16(lo, v);
+        hv_e4m3_to_bf16(hi, v + 2);
+    }
+};
+HV_DEV hv_i32x8 hv_join32(u32x4 lo, u32x4 hi) {
+    return hv_i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+template <>
+HV_DEV void HvFp8Frag<false>::set(u32x4 lo, u32x4 hi) {
+    v = hv_join32(lo, hi);
+}
+HV_DEV f32x4 hv_fp8_block_product(const HvFp8Frag<false>& a, const HvFp8Frag<false>& b) { return hv_mfma_fp8_128(a.v, b.v); }
+HV_DEV f32x4 hv_fp8_block_product(const HvFp8Frag<true>& a, const HvFp8Frag<true>& b) {
+    f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], c, 0, 0, 0);
+    return c;
+}
+
+struct HvGemmFp8Args {
+    hv_gemm_fp8_params p;
+    int kb;               // blocks of the reduction
+    int tiles_m, tiles_n;
+    int vec;              // Y and the residual take 16-byte accesses
+};
+
+// 16 consecutive columns n .. n + 15 of row m: bias, residual, rounding, store
+HV_DEV void hv_gemm_fp8_store(const HvGemmFp8Args& a, int m, int n, float* v) {
+    const hv_gemm_fp8_params& p = a.p;
+    if (a.vec && n + 16 <= p.N) {
+        if (p.residual) {
+            const bf16_t* r = p.residual + (long)m * p.ldr + n;
+            float f[16];
+            hv_unpack8(hv_ld16(r), f);
+            hv_unpack8(hv_ld16(r + 8), f + 8);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] += f[i];
+        }
+        if (p.out_f32) {
+            float* y = (float*)p.Y + (long)m * p.ldy + n;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4*>(y + 4 * i) = f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        } else {
+            bf16_t* y = (bf16_t*)p.Y + (long)m * p.ldy + n;
+            hv_st16(y, hv_pack8(v));
+            hv_st16(y + 8, hv_pack8(v + 8));
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if (n + i >= p.N) break;
+        float x = v[i];
+        if (p.residual) x += hv_bf2f(p.residual[(long)m * p.ldr + n + i]);
+        if (p.out_f32) ((float*)p.Y)[(long)m * p.ldy + n + i] = x;
+        else ((bf16_t*)p.Y)[(long)m * p.ldy + n + i] = hv_f2bf(x);
+    }
+}
+
+// ---- tiles: WM x WN waves, a wave computes 16 MT rows x 64 columns; two LDS stages of one 128-block each, filled by LDS-DMA.
+// LDS rows are 128 bytes (one block), their 16-byte pieces XOR-swizzled on the source side: X by (row >> 1) & 7; W, whose 16
+// rows of an MFMA are {16 q + 4 t + r}, by (row >> 1 & 1) | (row >> 4 & 3) << 1 -- both leave the 16 lanes of a ds_read_b128 on
+// 16 different quarters of the 64 banks.  The pieces behind K in the last block hold repeated values of the same row; their X
+// side is zeroed in registers.
+template <int WM, int WN, int MT, bool WIDE>
+__global__ __launch_bounds__(64 * WM * WN, 2) void hv_gemm_fp8_kernel(HvGemmFp8Args a) {
+    constexpr int BM = WM * MT * 16, BN = WN * 64, T = 64 * WM * WN, WAVES = WM * WN;
+    constexpr int XB = BM * 128, WB = BN * 128;
+    constexpr int XI = XB / 1024 / WAVES, WI = WB / 1024 / WAVES;  // DMA instructions (1024 bytes) per wave and stage
+    static_assert(XI * WAVES * 1024 == XB && WI * WAVES * 1024 == WB, "whole instructions per wave");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * (XB + WB)];
+    const hv_gemm_fp8_params& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+#ifndef HV_EMU
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#else
+    const int wave = tid >> 6;
+#endif
+    const int wm = wave % WM, wn = wave / WM;
+
+    // an XCD takes a contiguous range of tiles; inside it groups of 8 row tiles, the row tiles of a column tile adjacent: the
+    // 32 tiles in flight share 8 panels of X and 4 of W in its L2
+    const int total = a.tiles_m * a.tiles_n, per_xcd = (total + 7) / 8;
+    const int t = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per_xcd || t >= total) return;
+    const int grp = t / (8 * a.tiles_n), in_grp = t % (8 * a.tiles_n);
+    const int gm = min(8, a.tiles_m - grp * 8);
+    const int m0 = (grp * 8 + in_grp % gm) * BM, n0 = in_grp / gm * BN;
+
+    // DMA sources: instruction i of the tile carries rows 8 i .. 8 i + 7, lane l the piece (l & 7) ^ key(row) of row 8 i + l / 8;
+    // rows past the end repeat the last row (their products are never stored)
+    const char* const xbase = (const char*)p.X + (long)m0 * p.ldx;
+    const char* const wbase = (const char*)p.W + (long)n0 * p.ldw;
+    unsigned xofs[XI], wofs[WI];
+    int xpiece[XI], wpiece[WI];
+#pragma unroll
+    for (int i = 0; i < XI; ++i) {
+        const int row = (wave * XI + i) * 8 + (lane >> 3);
+        xpiece[i] = ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+        xofs[i] = (unsigned)min(row, p.M - 1 - m0) * (unsigned)p.ldx;
+    }
+#pragma unroll
+    for (int i = 0; i < WI; ++i) {
+        const int row = (wave * WI + i) * 8 + (lane >> 3);
+        wpiece[i] = ((lane & 7) ^ (((row >> 1) & 1) | (((row >> 4) & 3) << 1))) * 16;
+        wofs[i] = (unsigned)min(row, p.N - 1 - n0) * (unsigned)p.ldw;
+    }
+    auto issue = [&](int kb, int st) {
+        unsigned char* xs = smem + st * (XB + WB);
+        unsigned char* ws = xs + XB;
+        const int left = p.K - kb * 128 - 16;  // last piece inside K
+#pragma unroll
+        for (int i = 0; i < XI; ++i) hv_glds16_s(xbase + (long)kb * 128, xofs[i] + (unsigned)min(xpiece[i], left), xs + (wave * XI + i) * 1024);
+#pragma unroll
+        for (int i = 0; i < WI; ++i) hv_glds16_s(wbase + (long)kb * 128, wofs[i] + (unsigned)min(wpiece[i], left), ws + (wave * WI + i) * 1024);
+    };
+
+    const float* xsp[MT];
+    float xnext[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        xsp[i] = p.x_scale + (long)min(m0 + (wm * MT + i) * 16 + col, p.M - 1) * p.x_scale_row;
+        xnext[i] = xsp[i][0];
+    }
+    const float* wsp = p.w_scale + (long)(min(n0 + wn * 64, p.N - 1) / 128) * p.w_scale_row;
+    f32x4 acc[4][MT];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    issue(0, 0);
+    for (int kb = 0; kb < a.kb; ++kb) {
+        const int st = kb & 1;
+        float f[MT];
+        const float wsc = wsp[(long)kb * p.w_scale_k];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) f[i] = xnext[i] * wsc;
+        hv_vm_wait<0>();
+        hv_barrier_raw();  // block kb has landed, and nobody reads the other stage any more
+        if (kb + 1 < a.kb) {
+            issue(kb + 1, st ^ 1);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xnext[i] = xsp[i][(long)(kb + 1) * p.x_scale_k];
+        }
+        const unsigned char* xs = smem + st * (XB + WB);
+        const unsigned char* ws = xs + XB;
+        const int left = p.K - kb * 128;
+        HvFp8Frag<WIDE> wf[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = wn * 64 + (col >> 2) * 16 + i * 4 + (col & 3);
+            const int key = ((row >> 1) & 1) | (((row >> 4) & 3) << 1);
+            wf[i].set(hv_ld16(ws + row * 128 + ((g ^ key) << 4)), hv_ld16(ws + row * 128 + (((g + 4) ^ key) << 4)));
+        }
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            const int row = (wm * MT + j) * 16 + col, key = (row >> 1) & 7;
+            u32x4 lo = hv_ld16(xs + row * 128 + ((g ^ key) << 4)), hi = hv_ld16(xs + row * 128 + (((g + 4) ^ key) << 4));
+            if (left < 128) {
+                const u32x4 zero4 = {0u, 0u, 0u, 0u};
+                if (g * 16 >= left) lo = zero4;
+                if (g * 16 + 64 >= left) hi = zero4;
+            }
+            HvFp8Frag<WIDE> xf;
+            xf.set(lo, hi);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 part = hv_fp8_block_product(wf[i], xf);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(part[r], f[j], acc[i][j][r]);
+            }
+        }
+    }
+
+    const int n = n0 + wn * 64 + g * 16;
+    float bias[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bias[i] = p.bias && n + i < p.N ? p.bias[n + i] : 0.f;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        const int m = m0 + (wm * MT + j) * 16 + col;
+        if (m >= p.M || n >= p.N) continue;
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = acc[i / 4][j][i % 4] + bias[i];
+        hv_gemm_fp8_store(a, m, n, v);
+    }
+}
+
+// ---- few rows (M <= 16 MT): the weights' bytes are what counts.  A workgroup takes 16 columns; its eight waves take the blocks
+// of the reduction in turn, operands straight from memory into registers, and their sums are joined in LDS.
+template <int MT, bool WIDE>
+__global__ __launch_bounds__(512) void hv_gemm_fp8_rows_kernel(HvGemmFp8Args a) {
+    __shared__ __attribute__((aligned(16))) float red[8][MT][64][4];
+    const hv_gemm_fp8_params& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const unsigned char* wp = p.W + (long)min(n0 + col, p.N - 1) * p.ldw;
+    const float* wsp = p.w_scale + (long)(n0 / 128) * p.w_scale_row;
+    const unsigned char* xp[MT];
+    const float* xsp[MT];
+    f32x4 acc[MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        const int m = min(j * 16 + col, p.M - 1);
+        xp[j] = p.X + (long)m * p.ldx;
+        xsp[j] = p.x_scale + (long)m * p.x_scale_row;
+        acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int kb = wave; kb < a.kb; kb += 8) {
+        const int k = kb * 128 + g * 32, k1 = min(k, p.K - 16), k2 = min(k + 16, p.K - 16);
+        const u32x4 zero4 = {0u, 0u, 0u, 0u};
+        HvFp8Frag<WIDE> wf;
+        wf.set(hv_ld16(wp + k1), hv_ld16(wp + k2));
+        const float wsc = wsp[(long)kb * p.w_scale_k];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            HvFp8Frag<WIDE> xf;
+            xf.set(k < p.K ? hv_ld16(xp[j] + k1) : zero4, k + 16 < p.K ? hv_ld16(xp[j] + k2) : zero4);
+            const float f = xsp[j][(long)kb * p.x_scale_k] * wsc;
+            const f32x4 part = hv_fp8_block_product(wf, xf);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(part[r], f, acc[j][r]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(red[wave][j][lane]) = acc[j];
+    __syncthreads();
+    for (int i = tid; i < MT * 256; i += 512) {
+        const int j = i / 256, r = i % 16, c = i / 16 % 16;  // row m = 16 j + c, column n0 + r: neighbouring threads, neighbouring columns
+        const int m = j * 16 + c, n = n0 + r;
+        if (m >= p.M || n >= p.N) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) v += red[w][j][(r / 4) * 16 + c][r % 4];
+        if (p.bias) v += p.bias[n];
+        if (p.residual) v += hv_bf2f(p.residual[(long)m * p.ldr + n]);
+        if (p.out_f32) ((float*)p.Y)[(long)m * p.ldy + n] = v;
+        else ((bf16_t*)p.Y)[(long)m * p.ldy + n] = hv_f2bf(v);
+    }
+}
+
+static inline long hv_gemm_fp8_workspace_of(const hv_gemm_fp8_params& p) {
+    if (p.M < 0 || p.N < 0 || p.K < 16 || p.K % 16 != 0) return -1;
+    return 0;
+}
+
+static int g_hv_gemm_fp8_tile = 0;  // hv_set_tuning(HV_TUNE_GEMM_FP8)
+
+static inline int hv_gemm_fp8_launch(const hv_gemm_fp8_params& p, hipStream_t stream) {
+    if (p.M < 0 || p.N < 0 || p.K < 16 || p.K % 16 != 0 || p.ldx % 16 != 0 || p.ldw % 16 != 0) return -1;
+    if ((((uint64_t)p.X | (uint64_t)p.W) & 15) != 0) return -1;
+    if (p.ldx < 0 || p.ldw < 0 || p.ldx > (1L << 23) || p.ldw > (1L << 23)) return -1;  // 256 rows within 32-bit offsets
+    if (p.M == 0 || p.N == 0) return 0;
+    HvGemmFp8Args a;
+    a.p = p;
+    a.kb = (p.K + 127) / 128;
+    const int esz = p.out_f32 ? 4 : 2;
+    a.vec = ((uint64_t)p.Y & 15) == 0 && (p.ldy * esz) % 16 == 0 && (!p.residual || (((uint64_t)p.residual & 15) == 0 && p.ldr % 8 == 0));
+    if (p.M <= 64) {
+        a.tiles_m = 1;
+        a.tiles_n = (p.N + 15) / 16;
+        hv_note("hv_gemm_fp8_rows_kernel | M=%d N=%d K=%d", p.M, p.N, p.K);
+        const dim3 grid((unsigned)a.tiles_n), block(512);
+        auto go = [&](auto wide) {
+            constexpr bool WIDE = decltype(wide)::value;
+            if (p.M <= 16) hv_launch(hv_gemm_fp8_rows_kernel<1, WIDE>, grid, block, stream, a);
+            else if (p.M <= 32) hv_launch(hv_gemm_fp8_rows_kernel<2, WIDE>, grid, block, stream, a);
+            else hv_launch(hv_gemm_fp8_rows_kernel<4, WIDE>, grid, block, stream, a);
+        };
+        if (p.out_f32) go(std::true_type{});
+        else go(std::false_type{});
+        return 0;
+    }
+    auto tiles = [&](int bm, int bn) { return (long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+    auto set = [&](int bm, int bn) {
+        a.tiles_m = (p.M + bm - 1) / bm;
+        a.tiles_n = (p.N + bn - 1) / bn;
+        return dim3((unsigned)((tiles(bm, bn) + 7) / 8 * 8));
+    };
+    if (tiles(64, 64) > 0x3fffffffL) return -1;
+    if (g_hv_gemm_fp8_tile == 256 || (g_hv_gemm_fp8_tile == 0 && tiles(256, 256) >= 256)) {
+        const dim3 grid = set(256, 256);
+        hv_note("hv_gemm_fp8_kernel<2,4,8> | M=%d N=%d K=%d", p.M, p.N, p.K);
+        if (p.out_f32) hv_launch(hv_gemm_fp8_kernel<2, 4, 8, true>, grid, dim3(512), stream, a);
+        else hv_launch(hv_gemm_fp8_kernel<2, 4, 8, false>, grid, dim3(512), stream, a);
+    } else if (g_hv_gemm_fp8_tile == 128 || (g_hv_gemm_fp8_tile == 0 && tiles(128, 128) >= 256)) {
+        const dim3 grid = set(128, 128);
+        hv_note("hv_gemm_fp8_kernel<2,2,4> | M=%d N=%d K=%d", p.M, p.N, p.K);
+        if (p.out_f32) hv_launch(hv_gemm_fp8_kernel<2, 2, 4, true>, grid, dim3(256), stream, a);
+        else hv_launch(hv_gemm_fp8_kernel<2, 2, 4, false>, grid, dim3(256), stream, a);
+    } else {
+        const dim3 grid = set(64, 64);
+        hv_note("hv_gemm_fp8_kernel<4,1,1> | M=%d N=%d K=%d", p.M, p.N, p.K);
+        if (p.out_f32) hv_launch(hv_gemm_fp8_kernel<4, 1, 1, true>, grid, dim3(256), stream, a);
+        else hv_launch(hv_gemm_fp8_kernel<4, 1, 1, false>, grid, dim3(256), stream, a);
+    }
+    return 0;
+}
+
+// ---- quantisation to e4m3 with a scale for each 1 x 128 (block_rows 1: activations) or 128 x 128 block (weights) -----------------
+//   s = max(max|x| / 448, 2^-126), 1 for a block of zeros;  q = the e4m3 value nearest to x 448 / max|x| (ties to even).
+// The quotient of two bf16 numbers often lies exactly between two e4m3 values, and x * (448 / max|x|) in fp32 may miss such a
+// middle by its rounding (2^-23).  x 448 / max|x| is a quotient of integers below 2^11 and 2^8: it is on a middle (at most 5
+// significant bits) or at least 2^-13 away from it, relatively.  Rounding the product to 16 significant bits before the
+// conversion therefore gives the conversion of the exact quotient.
+HV_DEV float hv_row16_max(float x) {
+#ifndef HV_EMU
+    x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0xB1, 0xf, 0xf, true)));
+    x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x4E, 0xf, 0xf, true)));
+    x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x141, 0xf, 0xf, true)));
+    x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x140, 0xf, 0xf, true)));
+#else
+    for (int o = 1; o < 16; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
+#endif
+    return x;
+}
+HV_DEV float hv_amax8(u32x4 v) {  // max |x| of 8 bf16 (a NaN is passed over: it does not set a scale)
+    float f[8];
+    hv_unpack8(v, f);
+    float m = fabsf(f[0]);
+#pragma unroll
+    for (int e = 1; e < 8; ++e) m = fmaxf(m, fabsf(f[e]));
+    return fmaxf(m, 0.f);
+}
+HV_DEV float hv_fp8_block_scale(float amax, float& inv) {
+    const float s = amax / 448.0f;
+    if (amax == 0.f) {
+        inv = 1.f;
+        return 1.f;
+    }
+    if (s < 1.17549435e-38f) {  // 2^-126, the smallest normal number
+        inv = 8.50705917e37f;   // 2^126
+        return 1.17549435e-38f;
+    }
+    inv = 448.0f / amax;
+    return s;
+}
+HV_DEV u32x2 hv_quant8(u32x4 v, float inv) {
+    float f[8];
+    hv_unpack8(v, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, f[e] * inv);
+        f[e] = __builtin_bit_cast(float, (u + 0x80u) & ~0xffu);
+    }
+    return u32x2{hv_e4m3x4(f), hv_e4m3x4(f + 4)};
+}
+
+struct HvQuantArgs {
+    const bf16_t* X;
+    unsigned char* Q;
+    float* scale;
+    long ldx, ldq, scale_row, scale_k;
+    int M, K, kb;
+};
+
+// one scale per row and block: 16 lanes per (row, block), 16 bytes per lane
+__global__ __launch_bounds__(256) void hv_fp8_quantize_rows_kernel(HvQuantArgs a) {
+    const int lane16 = threadIdx.x & 15;
+    const long items = (long)a.M * a.kb;
+    const long i = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const bool live = i < items;  // no early return: every lane takes part in the reduction below
+    const long row = live ? i / a.kb : 0;
+    const int blk = live ? (int)(i % a.kb) : 0;
+    const int k = blk * 128 + lane16 * 8;
+    const bool on = live && k < a.K;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (on) v = hv_ld16(a.X + row * a.ldx + k);
+    const float amax = hv_row16_max(hv_amax8(v));
+    float inv;
+    const float s = hv_fp8_block_scale(amax, inv);
+    if (on) hv_st8(a.Q + row * a.ldq + k, hv_quant8(v, inv));
+    if (live && lane16 == 0) a.scale[row * a.scale_row + (long)blk * a.scale_k] = s;
+}
+
+// one scale per 128 x 128 block: a workgroup holds the block in registers
+__global__ __launch_bounds__(256) void hv_fp8_quantize_blocks_kernel(HvQuantArgs a) {
+    __shared__ float top[4];
+    const int tid = threadIdx.x, blk = blockIdx.x, m0 = blockIdx.y * 128;
+    const int k = blk * 128 + (tid & 15) * 8;
+    u32x4 v[8];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int row = m0 + i * 16 + (tid >> 4);
+        v[i] = u32x4{0u, 0u, 0u, 0u};
+        if (row < a.M && k < a.K) v[i] = hv_ld16(a.X + (long)row * a.ldx + k);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, hv_amax8(v[i]));
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+    if ((tid & 63) == 0) top[tid >> 6] = amax;
+    __syncthreads();
+    amax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    float inv;
+    const float s = hv_fp8_block_scale(amax, inv);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int row = m0 + i * 16 + (tid >> 4);
+        if (row < a.M && k < a.K) hv_st8(a.Q + (long)row * a.ldq + k, hv_quant8(v[i], inv));
+    }
+    if (tid == 0) a.scale[(long)blockIdx.y * a.scale_row + (long)blk * a.scale_k] = s;
+}
+
+static inline int hv_fp8_quantize_launch(const HvQuantArgs& in, int block_rows, hipStream_t stream) {
+    HvQuantArgs a = in;
+    if (a.M < 0 || a.K <= 0 || a.K % 16 != 0 || a.ldx % 8 != 0 || a.ldq % 16 != 0 || (block_rows != 1 && block_rows != 128)) return -1;
+    if ((((uint64_t)a.X | (uint64_t)a.Q) & 15) != 0) return -1;
+    if (a.M == 0) return 0;
+    a.kb = (a.K + 127) / 128;
+    if (block_rows == 1) {
+        const long wgs = ((long)a.M * a.kb + 15) / 16;
+        if (wgs > 0x7fffffffL) return -1;
+        hv_note("hv_fp8_quantize_rows_kernel | M=%d K=%d", a.M, a.K);
+        hv_launch(hv_fp8_quantize_rows_kernel, dim3((unsigned)wgs), dim3(256), stream, a);
+    } else {
+        if ((a.M + 127) / 128 > 65535) return -1;
+        hv_note("hv_fp8_quantize_blocks_kernel | M=%d K=%d", a.M, a.K);
+        hv_launch(hv_fp8_quantize_blocks_kernel, dim3((unsigned)a.kb, (unsigned)((a.M + 127) / 128)), dim3(256), stream, a);
+    }
+    return 0;
+}

@@ -30,6 +30,13 @@ int hvk_attention_fp8_quantize(const bf16_t* K, long ldk, const bf16_t* Vt, long
                                int phase, hipStream_t s);
 int hvk_attention_fp8(const hv_attention_params& p, const float* ks, const float* va, const float* ks2, const float* va2,
                       hipStream_t s);
+int hvk_cross_attention(const hv_cross_attention_params& p, hipStream_t s);
+long hvk_cross_attention_workspace(const hv_cross_attention_params& p);
+int hvk_gemm_fp8(const hv_gemm_fp8_params& p, hipStream_t s);
+void hvk_gemm_fp8_tile(int v);
+long hvk_gemm_fp8_workspace(const hv_gemm_fp8_params& p);
+int hvk_fp8_quantize(const bf16_t* X, long ldx, int M, int K, int block_rows, unsigned char* Q, long ldq, float* scale, long scale_row,
+                     long scale_k, hipStream_t s);
 int hvk_temporal(const hv_temporal_attention_params& p, hipStream_t s);
 void hvk_pack(const void* src, int src_bf16, int B, int C, int Fsrc, int H, int W, const int* frames, int F, int rep,
               bf16_t* dst, int Cpad, hipStream_t s);
@@ -51,4 +58,6 @@ void hvk_affine_apply(const bf16_t* X, long ldx, int rows, int rows_per_image, i
 #include "k_attention.hip"
 #include "k_temporal.hip"
 #include "k_elementwise.hip"
+#include "k_cross.hip"
+#include "k_fp8.hip"
 #endif

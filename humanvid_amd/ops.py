@@ -161,6 +161,115 @@ def attention_fp8(lib, stream, q, k, vt, o, kscale, vamax, *, n_images, heads, D
     lib.call("hv_attention_fp8", C.byref(p), _p(kscale), _p(vamax), _p(kscale2), _p(vamax2), stream)
 
 
+def _on_current_device(what, *tensors):
+    """the launch goes to the current device: every tensor has to be there"""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: tensors on {dev}, the current device is {torch.cuda.current_device()}")
+
+
+def cross_attention(lib, stream, q, k, v, o, *, heads, kv_heads=None, kv_len=None, key_mask=None, scale=None, workspace=None,
+                    query_workspace=False):
+    """o[b, i] = softmax(scale q[b, i] . k[b, j]) v[b, j] per head, over the attended states j: j < kv_len[b], key_mask[b, j] != 0.
+    q, o [B, Lq, heads * D], k, v [B, Lk, kv_heads * D] bf16 views (last dimension contiguous, other strides multiples of 8; k, v may be
+    expanded over the batch); heads // kv_heads query heads share a key head.  kv_len int32 [B], key_mask uint8 / bool [B, Lk] on the
+    device.  An entry that attends to nothing gets zeros.  scale: 1 / sqrt(D) by default.  o may be q.
+    query_workspace=True launches nothing and returns the fp32 elements `workspace` needs for these sizes (0: none)."""
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or o.shape != q.shape:
+        raise ValueError("cross_attention: q, o [B, Lq, heads * D] and k, v [B, Lk, kv_heads * D] expected")
+    B, Lq, Cq = q.shape
+    Lk = k.shape[1]
+    KH = heads if kv_heads is None else kv_heads
+    if heads <= 0 or KH <= 0 or Cq % heads or k.shape[0] != B or k.shape[2] != Cq // heads * KH:
+        raise ValueError(f"cross_attention: q {tuple(q.shape)}, k {tuple(k.shape)} do not fit {heads} heads, {KH} key heads")
+    if q.dtype != BF16 or k.dtype != BF16 or v.dtype != BF16 or o.dtype != BF16:
+        raise ValueError("cross_attention: q, k, v, o must be bfloat16")
+    D = Cq // heads
+    sq, sk, sv, so = q.stride(), k.stride(), v.stride(), o.stride()
+    if Cq > 1 and (sq[2] != 1 or so[2] != 1 or sk[2] != 1 or sv[2] != 1):
+        raise ValueError("cross_attention: the last dimension must be contiguous")
+    ms = 0
+    if kv_len is not None and (kv_len.dtype != torch.int32 or kv_len.shape != (B,) or not kv_len.is_contiguous()):
+        raise ValueError("cross_attention: kv_len must be contiguous int32 [B]")
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.uint8, torch.bool) or key_mask.shape != (B, Lk) or (Lk > 1 and key_mask.stride(1) != 1):
+            raise ValueError("cross_attention: key_mask must be uint8 or bool [B, Lk], its last dimension contiguous")
+        ms = key_mask.stride(0)
+    if workspace is not None and (workspace.dtype != torch.float32 or not workspace.is_contiguous()):
+        raise ValueError("cross_attention: workspace must be contiguous float32")
+    p = A.CrossAttentionParams(
+        q.data_ptr(), sq[1], sq[0], k.data_ptr(), sk[1], sk[0], v.data_ptr(), sv[1], sv[0], o.data_ptr(), so[1], so[0],
+        _p(kv_len), _p(key_mask), ms, B, Lq, Lk, heads, KH, D, 1.0 / math.sqrt(D) if scale is None else scale,
+        _p(workspace), 0 if workspace is None else workspace.numel())
+    if query_workspace:
+        n = lib.cdll.hv_cross_attention_workspace(C.byref(p))
+        if n < 0:
+            lib.check(n)
+        return n
+    _on_current_device("cross_attention", q, k, v, o, kv_len, key_mask, workspace)
+    lib.call("hv_cross_attention", C.byref(p), stream)
+
+
+FP8 = (torch.float8_e4m3fn, torch.uint8)  # e4m3 values, by their own type or as bytes
+
+
+def fp8_quantize(lib, stream, x, q, scale, *, block_rows=1):
+    """x [M, K] bf16 -> q [M, K] e4m3 (float8_e4m3fn or uint8) and scale [ceil(M / block_rows), ceil(K / 128)] fp32 (any strides), one
+    scale per block_rows x 128 block: block_rows 1 for activations, 128 for weights.  x / scale to the nearest e4m3, ties to even.
+    A scale laid out [blocks, M] and passed transposed is what gemm_fp8 reads best."""
+    if x.dim() != 2 or q.shape != x.shape or block_rows not in (1, 128):
+        raise ValueError("fp8_quantize: x, q [M, K] and block_rows 1 or 128 expected")
+    M, K = x.shape
+    if x.dtype != BF16 or q.dtype not in FP8 or scale.dtype != torch.float32:
+        raise ValueError("fp8_quantize: x bfloat16, q float8_e4m3fn or uint8, scale float32 expected")
+    if scale.shape != (-(-M // block_rows), -(-K // 128)):
+        raise ValueError(f"fp8_quantize: scale {tuple(scale.shape)}, expected {(-(-M // block_rows), -(-K // 128))}")
+    if (K > 1 and (x.stride(1) != 1 or q.stride(1) != 1)) or (M > 1 and q.stride(0) < K):
+        raise ValueError("fp8_quantize: the rows of x and q must be contiguous, those of q must not overlap")
+    _on_current_device("fp8_quantize", x, q, scale)
+    lib.call("hv_fp8_quantize", x.data_ptr(), x.stride(0), M, K, block_rows, q.data_ptr(), q.stride(0), scale.data_ptr(),
+             scale.stride(0), scale.stride(1), stream)
+
+
+def gemm_fp8(lib, stream, x, x_scale, w, w_scale, y, *, bias=None, residual=None, workspace=None, query_workspace=False):
+    """y[M, N] = (x * x_scale) @ (w * w_scale)^T + bias + residual, x [M, K], w [N, K] e4m3 (float8_e4m3fn or uint8), x_scale
+    [M, ceil(K / 128)], w_scale [ceil(N / 128), ceil(K / 128)] fp32 (any strides), y bf16 or fp32, bias fp32 [N], residual bf16 [M, N]
+    (may be y).  K a multiple of 16; x / w / y / residual may be row-strided views.
+    query_workspace=True launches nothing and returns the fp32 elements `workspace` needs for these sizes (0: none)."""
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or y.shape != (x.shape[0], w.shape[0]):
+        raise ValueError("gemm_fp8: x [M, K], w [N, K], y [M, N] expected")
+    M, K = x.shape
+    N = w.shape[0]
+    kb = -(-K // 128)
+    if x.dtype not in FP8 or w.dtype not in FP8 or y.dtype not in (BF16, torch.float32):
+        raise ValueError("gemm_fp8: x, w float8_e4m3fn or uint8, y bfloat16 or float32 expected")
+    if x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32 or x_scale.shape != (M, kb) or w_scale.shape != (-(-N // 128), kb):
+        raise ValueError(f"gemm_fp8: float32 x_scale {(M, kb)} and w_scale {(-(-N // 128), kb)} expected, got {tuple(x_scale.shape)}, {tuple(w_scale.shape)}")
+    if (K > 1 and (x.stride(1) != 1 or w.stride(1) != 1)) or (N > 1 and y.stride(1) != 1) or (M > 1 and y.stride(0) < N):
+        raise ValueError("gemm_fp8: the rows of x, w and y must be contiguous, those of y must not overlap")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or not bias.is_contiguous()):
+        raise ValueError("gemm_fp8: bias must be contiguous float32 [N]")
+    if residual is not None and (residual.dtype != BF16 or residual.shape != y.shape or (N > 1 and residual.stride(1) != 1)):
+        raise ValueError("gemm_fp8: residual must be bfloat16 [M, N] with contiguous rows")
+    if workspace is not None and (workspace.dtype != torch.float32 or not workspace.is_contiguous()):
+        raise ValueError("gemm_fp8: workspace must be contiguous float32")
+    p = A.GemmFp8Params(
+        x.data_ptr(), x.stride(0), x_scale.data_ptr(), x_scale.stride(0), x_scale.stride(1), w.data_ptr(), w.stride(0),
+        w_scale.data_ptr(), w_scale.stride(0), w_scale.stride(1), y.data_ptr(), y.stride(0), y.dtype == torch.float32, M, N, K,
+        _p(bias), _p(residual), 0 if residual is None else residual.stride(0), _p(workspace),
+        0 if workspace is None else workspace.numel())
+    if query_workspace:
+        n = lib.cdll.hv_gemm_fp8_workspace(C.byref(p))
+        if n < 0:
+            lib.check(n)
+        return n
+    _on_current_device("gemm_fp8", x, x_scale, w, w_scale, y, bias, residual, workspace)
+    lib.call("hv_gemm_fp8", C.byref(p), stream)
+
+
 def temporal_attention(lib, stream, qkv, o, *, B, F, P, heads, D):
     """Single-device form: qkv [(B F P), 3C] rows (b*F + f)*P + p with columns [q | k | v]."""
     Cc = heads * D

@@ -217,6 +217,66 @@ int hv_attention_fp8_quantize(const uint16_t* K, long ldk, const uint16_t* Vt, l
 int hv_attention_fp8(const hv_attention_params* p, const float* kscale, const float* vamax, const float* kscale2,
                      const float* vamax2, void* stream);
 
+/* ---- cross attention: Lq queries per batch entry to Lk encoder states ------------------------------------------------
+ * The UNets' attn2 when encoder_hidden_states has more than one token (src/models/attention.py:410-424, diffusers Attention):
+ * O[b][i][h] = sum_j softmax_j(scale Q[b][i][h] . K[b][j][g]) V[b][j][g],  g = h / (heads / kv_heads), over the attended states:
+ * j < kv_len[b] and key_mask[b][j] != 0.  A batch entry with no attended state gets zeros; what memory holds in the other
+ * states (NaN included) does not reach the output, and states at or behind kv_len are not read.  Values are row-major.  All frames of a
+ * clip that share their half's prompt are ONE batch entry (Lq = frames * tokens).  O may be Q.  Any Lq, Lk >= 0; D in
+ * {40, 64, 80, 128, 160}; pointers 16-byte aligned, strides multiples of 8 elements (the batch strides of K, V and the mask may be 0:
+ * shared states).  The keys are cut into ranges that are joined by a second launch where the queries alone would not fill the
+ * chip: hv_cross_attention_workspace() floats of scratch, not to be shared by calls that may run at the same time. */
+typedef struct hv_cross_attention_params {
+    const uint16_t* Q; /* row i of entry b at Q + b * q_stride_b + i * ldq, head h at column h*D */
+    long ldq, q_stride_b;
+    const uint16_t* K; /* row j of entry b, key head g at column g*D */
+    long ldk, k_stride_b;
+    const uint16_t* V;
+    long ldv, v_stride_b;
+    uint16_t* O;
+    long ldo, o_stride_b;
+    const int* kv_len;       /* device [B] or NULL: Lk (values outside 0..Lk are clamped) */
+    const uint8_t* key_mask; /* device [B][Lk] bytes, row stride mask_stride_b, or NULL */
+    long mask_stride_b;
+    int B, Lq, Lk, heads, kv_heads, D;
+    float scale; /* > 0, finite */
+    float* workspace;
+    long workspace_floats;
+} hv_cross_attention_params;
+int hv_cross_attention(const hv_cross_attention_params* p, void* stream);
+long hv_cross_attention_workspace(const hv_cross_attention_params* p); /* floats hv_cross_attention needs for these sizes, negative on error */
+
+/* ---- projections in 8-bit floating point (OCP e4m3) with a scale for each block of 128 of the reduction -----------------
+ * hv_fp8_quantize: X [M][K] bf16 -> Q [M][K] e4m3 and one scale per block_rows x 128 block (block_rows 1: activations, 128:
+ * weights; blocks at the edges are shorter): scale = max(max|x| / 448, 2^-126), 1 for a block of zeros, Q = x 448 / max|x| to the
+ * nearest e4m3, ties to even (exactly: the quotient is not rounded before).  A NaN stays one and sets no scale; a block with an
+ * infinity is NaN as a whole.  scale element (row block i, column block j) at scale[i * scale_row + j * scale_k].
+ * hv_gemm_fp8: Y[m][n] = bias[n] + residual[m][n] + sum_kb x_scale[m][kb] w_scale[n/128][kb] (X . W^T over block kb), fp32 sums,
+ * rounded once.  K a multiple of 16 (the last block may be short), X, W, Q rows 16-byte aligned; any M, N >= 0. */
+int hv_fp8_quantize(const uint16_t* X, long ldx, int M, int K, int block_rows, uint8_t* Q, long ldq, float* scale, long scale_row,
+                    long scale_k, void* stream);
+typedef struct hv_gemm_fp8_params {
+    const uint8_t* X; /* e4m3 [M][K] */
+    long ldx;
+    const float* x_scale; /* element (m, kb) at x_scale[m * x_scale_row + kb * x_scale_k] */
+    long x_scale_row, x_scale_k;
+    const uint8_t* W; /* e4m3 [N][K] */
+    long ldw;
+    const float* w_scale; /* element (n / 128, kb) */
+    long w_scale_row, w_scale_k;
+    void* Y; /* bf16, or float when out_f32 */
+    long ldy;
+    int out_f32;
+    int M, N, K;
+    const float* bias;        /* [N] or NULL */
+    const uint16_t* residual; /* bf16 [M][N] or NULL; may be Y */
+    long ldr;
+    float* workspace;
+    long workspace_floats;
+} hv_gemm_fp8_params;
+int hv_gemm_fp8(const hv_gemm_fp8_params* p, void* stream);
+long hv_gemm_fp8_workspace(const hv_gemm_fp8_params* p); /* floats of scratch hv_gemm_fp8 needs for these sizes, negative on error */
+
 /* kernel-variant selection for A/B measurements (process-global; not needed for correctness) */
 #define HV_TUNE_ATTN_D40 0     /* head dim 40: 0 (default) = the dedicated 8-wave kernel (hv_attention40.h: 32x32x16 QK^T, 256 queries per workgroup); 2 = the generic kernel (A/B) */
 #define HV_TUNE_GEMM_MAX_GRID 2 /* persistent GEMM workgroups (multiple of 8, default 512) */
@@ -230,6 +290,7 @@ int hv_attention_fp8(const hv_attention_params* p, const float* kscale, const fl
 #define HV_TUNE_CONV_RASTER 9    /* workgroup raster of hv_conv3x3 inside an XCD: 0 = the output-channel tiles of a pixel patch adjacent (halo shared through L2, weights re-streamed), 1 = the pixel patches of an output-channel tile adjacent (weights stay in L2), 2 (default) = 1 where Cin x Cout >= 640 x 640: HBM-side fetch of the 1280 -> 1280 convolution 1.4 -> 0.6 GB per launch at equal time (profiles/r04_s3.txt) */
 #define HV_TUNE_CONV_W4 12       /* stride-1 convolutions of a plain single-source input with Cout % 320 == 0 or Cout % 256 == 0 on hv_conv_w4_kernel (hv_conv4.h: 12 x 16 pixels x 320 / 256 channels on four waves, halo and weights by LDS-DMA; the width whose tiles fill the rounds of 256 CUs better): 1 (default) = where the tiles fill their rounds of 256 CUs to >= 70 % (>= 128 tiles) and the patches cover >= 80 % of the image, 0 = never, 2 = wherever the structure allows (tests), 3 = as 1 with 320-channel tiles only (A/B) */
 #define HV_TUNE_CMDLIST_GRAPHS 7 /* 1 (default): hv_cmdlist_run replays a recorded segment as ONE captured HIP graph; 0: re-issues its launches one by one (A/B) */
+#define HV_TUNE_GEMM_FP8 16      /* hv_gemm_fp8 with M > 64: 0 (default) = the largest tile that still gives every CU one; 64 / 128 / 256 = square tiles of that size (tests) */
 int hv_set_tuning(int key, int value);
 
 /* ---- temporal self-attention over the frame axis ------------------------------------------

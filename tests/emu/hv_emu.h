@@ -306,6 +306,52 @@ inline hv_f4 mfma_fp8(long a, long b, hv_f4 c) {
     return out;
 }
 }  // namespace hvemu
+
+// v_mfma_f32_16x16x128_f8f6f4 on e4m3 operands: 32 values per lane, lane (i = lane & 15, g = lane >> 4) holds k = 32 g + 0..31
+// (the kernels give both operands the same lane -> k assignment, so the order inside the 128 does not matter to them)
+typedef int hv_i8x32 __attribute__((ext_vector_type(8)));
+namespace hvemu {
+inline hv_f4 mfma_fp8_128(hv_i8x32 a, hv_i8x32 b, hv_f4 c) {
+    struct In {
+        hv_i8x32 a, b;
+        hv_f4 c;
+    } in{a, b, c};
+    hv_f4 out;
+    wave_collective(&in, sizeof(in), &out, sizeof(out), [](WaveState& w) {
+        static float A[16][128], B[128][16];
+        static float table[256];
+        static bool made = false;
+        if (!made) {
+            for (int i = 0; i < 256; ++i) table[i] = fp8_to_f((unsigned char)i);
+            made = true;
+        }
+        for (int l = 0; l < 64; ++l) {
+            In li;
+            memcpy(&li, w.in[l], sizeof(In));
+            unsigned char ab[32], bb[32];
+            memcpy(ab, &li.a, 32);
+            memcpy(bb, &li.b, 32);
+            for (int j = 0; j < 32; ++j) {
+                A[l % 16][(l / 16) * 32 + j] = table[ab[j]];
+                B[(l / 16) * 32 + j][l % 16] = table[bb[j]];
+            }
+        }
+        for (int l = 0; l < 64; ++l) {
+            In li;
+            memcpy(&li, w.in[l], sizeof(In));
+            hv_f4 o;
+            for (int r = 0; r < 4; ++r) {
+                const int col = l % 16, row = (l / 16) * 4 + r;
+                float acc = li.c[r];
+                for (int k = 0; k < 128; ++k) acc = fmaf(A[row][k], B[k][col], acc);
+                o[r] = acc;
+            }
+            memcpy(w.out[l], &o, sizeof(hv_f4));
+        }
+    });
+    return out;
+}
+}  // namespace hvemu
 inline int atomicMax(int* p, int v) {
     const int old = *p;
     if (v > old) *p = v;
