@@ -151,6 +151,15 @@ HV_DEV void hv_glds16_s(const void* base_uniform, unsigned byte_ofs, void* lds_w
                  : "v"(byte_ofs), "s"(base_uniform), "s"(lds_addr_uniform)
                  : "memory");
 }
+// the same with 4 bytes per lane (LDS destination: wave base + lane * 4)
+HV_DEV void hv_glds4_s(const void* base_uniform, unsigned byte_ofs, void* lds_wave_base) {
+    const unsigned lds_addr_uniform = (unsigned)(unsigned long)(__attribute__((address_space(3))) void*)lds_wave_base;
+    unsigned keep;
+    asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(byte_ofs), "s"(base_uniform), "s"(lds_addr_uniform)
+                 : "memory");
+}
 template <int N>
 HV_DEV void hv_vm_wait() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -165,6 +174,9 @@ HV_DEV void hv_glds16(const void* gsrc, void* lds_wave_base) {
 }
 HV_DEV void hv_glds16_s(const void* base_uniform, unsigned byte_ofs, void* lds_wave_base) {
     memcpy((char*)lds_wave_base + (threadIdx.x & 63) * 16, (const char*)base_uniform + byte_ofs, 16);
+}
+HV_DEV void hv_glds4_s(const void* base_uniform, unsigned byte_ofs, void* lds_wave_base) {
+    memcpy((char*)lds_wave_base + (threadIdx.x & 63) * 4, (const char*)base_uniform + byte_ofs, 4);
 }
 template <int N>
 HV_DEV void hv_vm_wait() {}

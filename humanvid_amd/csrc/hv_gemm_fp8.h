@@ -87,6 +87,12 @@ HV_DEV f32x4 hv_fp8_block_product(const HvFp8Frag<true>& a, const HvFp8Frag<true
     return c;
 }
 
+HV_DEV void hv_sched_fence() {  // the scheduler moves nothing across: keeps a software pipeline's registers bounded
+#ifndef HV_EMU
+    __builtin_amdgcn_sched_barrier(0);
+#endif
+}
+
 struct HvGemmFp8Args {
     hv_gemm_fp8_params p;
     int kb;               // blocks of the reduction
@@ -134,11 +140,11 @@ HV_DEV void hv_gemm_fp8_store(const HvGemmFp8Args& a, int m, int n, float* v) {
 // side is zeroed in registers.
 template <int WM, int WN, int MT, bool WIDE>
 __global__ __launch_bounds__(64 * WM * WN, 2) void hv_gemm_fp8_kernel(HvGemmFp8Args a) {
-    constexpr int BM = WM * MT * 16, BN = WN * 64, T = 64 * WM * WN, WAVES = WM * WN;
-    constexpr int XB = BM * 128, WB = BN * 128;
+    constexpr int BM = WM * MT * 16, BN = WN * 64, WAVES = WM * WN;
+    constexpr int XB = BM * 128, WB = BN * 128, SB = BM * 4;       // bytes of a stage: X, W, the rows' scales
     constexpr int XI = XB / 1024 / WAVES, WI = WB / 1024 / WAVES;  // DMA instructions (1024 bytes) per wave and stage
-    static_assert(XI * WAVES * 1024 == XB && WI * WAVES * 1024 == WB, "whole instructions per wave");
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * (XB + WB)];
+    static_assert(XI * WAVES * 1024 == XB && WI * WAVES * 1024 == WB && BM / 64 <= WAVES, "whole instructions per wave");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * (XB + WB + SB)];
     const hv_gemm_fp8_params& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
 #ifndef HV_EMU
@@ -157,41 +163,33 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void hv_gemm_fp8_kernel(HvGemmFp8A
     const int gm = min(8, a.tiles_m - grp * 8);
     const int m0 = (grp * 8 + in_grp % gm) * BM, n0 = in_grp / gm * BN;
 
-    // DMA sources: instruction i of the tile carries rows 8 i .. 8 i + 7, lane l the piece (l & 7) ^ key(row) of row 8 i + l / 8;
-    // rows past the end repeat the last row (their products are never stored)
+    // DMA sources: instruction I = wave + WAVES i of a tile carries rows 8 I .. 8 I + 7, lane l the piece (l & 7) ^ key(row) of row
+    // 8 I + l / 8; I has the same parity for every i and, with 4 waves, I / 2 one of two values mod 4.  Rows past the end repeat
+    // the last row (their products are never stored).
     const char* const xbase = (const char*)p.X + (long)m0 * p.ldx;
     const char* const wbase = (const char*)p.W + (long)n0 * p.ldw;
-    unsigned xofs[XI], wofs[WI];
-    int xpiece[XI], wpiece[WI];
+    const char* const sbase = (const char*)(p.x_scale + (long)m0 * p.x_scale_row);
+    const int xpiece = ((lane & 7) ^ ((4 * (wave & 1) + (lane >> 4)) & 7)) * 16;
+    const int wpiece = ((lane & 7) ^ (((lane >> 4) & 1) | (((wave >> 1) & 3) << 1))) * 16;  // i odd, 4 waves: ^ (2 << 1) * 16
+    unsigned xofs[XI], wofs[WI], sofs = 0;
 #pragma unroll
-    for (int i = 0; i < XI; ++i) {
-        const int row = (wave * XI + i) * 8 + (lane >> 3);
-        xpiece[i] = ((lane & 7) ^ ((row >> 1) & 7)) * 16;
-        xofs[i] = (unsigned)min(row, p.M - 1 - m0) * (unsigned)p.ldx;
-    }
+    for (int i = 0; i < XI; ++i) xofs[i] = (unsigned)min((wave + WAVES * i) * 8 + (lane >> 3), p.M - 1 - m0) * (unsigned)p.ldx;
 #pragma unroll
-    for (int i = 0; i < WI; ++i) {
-        const int row = (wave * WI + i) * 8 + (lane >> 3);
-        wpiece[i] = ((lane & 7) ^ (((row >> 1) & 1) | (((row >> 4) & 3) << 1))) * 16;
-        wofs[i] = (unsigned)min(row, p.N - 1 - n0) * (unsigned)p.ldw;
-    }
+    for (int i = 0; i < WI; ++i) wofs[i] = (unsigned)min((wave + WAVES * i) * 8 + (lane >> 3), p.N - 1 - n0) * (unsigned)p.ldw;
+    if (wave < BM / 64) sofs = (unsigned)min(tid, p.M - 1 - m0) * (unsigned)(p.x_scale_row * 4);
     auto issue = [&](int kb, int st) {
-        unsigned char* xs = smem + st * (XB + WB);
+        unsigned char* xs = smem + st * (XB + WB + SB);
         unsigned char* ws = xs + XB;
         const int left = p.K - kb * 128 - 16;  // last piece inside K
+        const unsigned xp = (unsigned)min(xpiece, left);
+        const unsigned wp[2] = {(unsigned)min(wpiece, left), (unsigned)min(WAVES == 4 ? wpiece ^ 64 : wpiece, left)};
 #pragma unroll
-        for (int i = 0; i < XI; ++i) hv_glds16_s(xbase + (long)kb * 128, xofs[i] + (unsigned)min(xpiece[i], left), xs + (wave * XI + i) * 1024);
+        for (int i = 0; i < XI; ++i) hv_glds16_s(xbase + (long)kb * 128, xofs[i] + xp, xs + (wave + WAVES * i) * 1024);
 #pragma unroll
-        for (int i = 0; i < WI; ++i) hv_glds16_s(wbase + (long)kb * 128, wofs[i] + (unsigned)min(wpiece[i], left), ws + (wave * WI + i) * 1024);
+        for (int i = 0; i < WI; ++i) hv_glds16_s(wbase + (long)kb * 128, wofs[i] + wp[i & 1], ws + (wave + WAVES * i) * 1024);
+        if (wave < BM / 64) hv_glds4_s(sbase + (long)kb * p.x_scale_k * 4, sofs, ws + WB + wave * 256);
     };
 
-    const float* xsp[MT];
-    float xnext[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        xsp[i] = p.x_scale + (long)min(m0 + (wm * MT + i) * 16 + col, p.M - 1) * p.x_scale_row;
-        xnext[i] = xsp[i][0];
-    }
     const float* wsp = p.w_scale + (long)(min(n0 + wn * 64, p.N - 1) / 128) * p.w_scale_row;
     f32x4 acc[4][MT];
 #pragma unroll
@@ -200,46 +198,54 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void hv_gemm_fp8_kernel(HvGemmFp8A
         for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     issue(0, 0);
+    float wnext = wsp[0];
     for (int kb = 0; kb < a.kb; ++kb) {
         const int st = kb & 1;
-        float f[MT];
-        const float wsc = wsp[(long)kb * p.w_scale_k];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) f[i] = xnext[i] * wsc;
+        const float wsc = wnext;
         hv_vm_wait<0>();
         hv_barrier_raw();  // block kb has landed, and nobody reads the other stage any more
         if (kb + 1 < a.kb) {
             issue(kb + 1, st ^ 1);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) xnext[i] = xsp[i][(long)(kb + 1) * p.x_scale_k];
+            wnext = wsp[(long)(kb + 1) * p.w_scale_k];
         }
-        const unsigned char* xs = smem + st * (XB + WB);
+        unsigned char* xs = smem + st * (XB + WB + SB);
         const unsigned char* ws = xs + XB;
+        const float* ss = reinterpret_cast<const float*>(ws + WB) + wm * MT * 16 + col;
         const int left = p.K - kb * 128;
-        HvFp8Frag<WIDE> wf[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = wn * 64 + (col >> 2) * 16 + i * 4 + (col & 3);
-            const int key = ((row >> 1) & 1) | (((row >> 4) & 3) << 1);
-            wf[i].set(hv_ld16(ws + row * 128 + ((g ^ key) << 4)), hv_ld16(ws + row * 128 + (((g + 4) ^ key) << 4)));
+        if (left < 128) {  // the last block is short: X is zero behind K
+            for (int i = tid; i < BM * 8; i += 64 * WAVES) {
+                const int row = i >> 3;
+                if ((i & 7) * 16 >= left) hv_st16(xs + row * 128 + (((i & 7) ^ ((row >> 1) & 7)) << 4), u32x4{0u, 0u, 0u, 0u});
+            }
+            __syncthreads();
         }
+        // fragments: row 16 j + col of the wave's X rows, key (col >> 1); row 16 (col / 4) + 4 i + col % 4 of its W rows
+        const unsigned char* const xrow = xs + (wm * MT * 16 + col) * 128;
+        const unsigned char* const wrow = ws + (wn * 64 + (col >> 2) * 16 + (col & 3)) * 128;
+        const int xk = (g ^ (col >> 1)) << 4, wk = (g ^ (((col >> 1) & 1) | ((col >> 2) << 1))) << 4;  // the second piece: ^ 64
+        HvFp8Frag<WIDE> wf[4], xf[2];
+        f32x4 part[2][4];
+        float f[2];
 #pragma unroll
-        for (int j = 0; j < MT; ++j) {
-            const int row = (wm * MT + j) * 16 + col, key = (row >> 1) & 7;
-            u32x4 lo = hv_ld16(xs + row * 128 + ((g ^ key) << 4)), hi = hv_ld16(xs + row * 128 + (((g + 4) ^ key) << 4));
-            if (left < 128) {
-                const u32x4 zero4 = {0u, 0u, 0u, 0u};
-                if (g * 16 >= left) lo = zero4;
-                if (g * 16 + 64 >= left) hi = zero4;
+        for (int i = 0; i < 4; ++i) wf[i].set(hv_ld16(wrow + i * 512 + wk), hv_ld16(wrow + i * 512 + (wk ^ 64)));
+        xf[0].set(hv_ld16(xrow + xk), hv_ld16(xrow + (xk ^ 64)));
+        f[0] = ss[0] * wsc;
+        // row tile j's products are in flight while row tile j - 1's are added up
+#pragma unroll
+        for (int j = 0; j <= MT; ++j) {
+            if (j + 1 < MT) xf[(j + 1) & 1].set(hv_ld16(xrow + (j + 1) * 2048 + xk), hv_ld16(xrow + (j + 1) * 2048 + (xk ^ 64)));
+            if (j < MT) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[j & 1][i] = hv_fp8_block_product(wf[i], xf[j & 1]);
             }
-            HvFp8Frag<WIDE> xf;
-            xf.set(lo, hi);
+            if (j > 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4 part = hv_fp8_block_product(wf[i], xf);
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(part[r], f[j], acc[i][j][r]);
+                    for (int r = 0; r < 4; ++r) acc[i][j - 1][r] = fmaf(part[(j - 1) & 1][i][r], f[(j - 1) & 1], acc[i][j - 1][r]);
             }
+            if (j + 1 < MT) f[(j + 1) & 1] = ss[(j + 1) * 16] * wsc;
+            hv_sched_fence();
         }
     }
 
@@ -322,6 +328,7 @@ static inline int hv_gemm_fp8_launch(const hv_gemm_fp8_params& p, hipStream_t st
     if (p.M < 0 || p.N < 0 || p.K < 16 || p.K % 16 != 0 || p.ldx % 16 != 0 || p.ldw % 16 != 0) return -1;
     if ((((uint64_t)p.X | (uint64_t)p.W) & 15) != 0) return -1;
     if (p.ldx < 0 || p.ldw < 0 || p.ldx > (1L << 23) || p.ldw > (1L << 23)) return -1;  // 256 rows within 32-bit offsets
+    if (p.x_scale_row < 0 || p.x_scale_row > (1L << 21)) return -1;
     if (p.M == 0 || p.N == 0) return 0;
     HvGemmFp8Args a;
     a.p = p;
@@ -350,12 +357,11 @@ static inline int hv_gemm_fp8_launch(const hv_gemm_fp8_params& p, hipStream_t st
         return dim3((unsigned)((tiles(bm, bn) + 7) / 8 * 8));
     };
     if (tiles(64, 64) > 0x3fffffffL) return -1;
-    if (g_hv_gemm_fp8_tile == 256 || (g_hv_gemm_fp8_tile == 0 && tiles(256, 256) >= 256)) {
+    if (!p.out_f32 && (g_hv_gemm_fp8_tile == 256 || (g_hv_gemm_fp8_tile == 0 && tiles(256, 256) >= 256))) {
         const dim3 grid = set(256, 256);
         hv_note("hv_gemm_fp8_kernel<2,4,8> | M=%d N=%d K=%d", p.M, p.N, p.K);
-        if (p.out_f32) hv_launch(hv_gemm_fp8_kernel<2, 4, 8, true>, grid, dim3(512), stream, a);
-        else hv_launch(hv_gemm_fp8_kernel<2, 4, 8, false>, grid, dim3(512), stream, a);
-    } else if (g_hv_gemm_fp8_tile == 128 || (g_hv_gemm_fp8_tile == 0 && tiles(128, 128) >= 256)) {
+        hv_launch(hv_gemm_fp8_kernel<2, 4, 8, false>, grid, dim3(512), stream, a);
+    } else if (g_hv_gemm_fp8_tile >= 128 || (g_hv_gemm_fp8_tile == 0 && tiles(128, 128) >= 256)) {
         const dim3 grid = set(128, 128);
         hv_note("hv_gemm_fp8_kernel<2,2,4> | M=%d N=%d K=%d", p.M, p.N, p.K);
         if (p.out_f32) hv_launch(hv_gemm_fp8_kernel<2, 2, 4, true>, grid, dim3(256), stream, a);
