@@ -47,14 +47,172 @@ struct HvCrossArgs {
     int groups;          // ceil(blocks / per_wg)
     int units;           // workgroups with work
     int splits;          // ranges the keys are cut into
+    int few, qt, np;     // which kernel; 16-row tiles per wave; pairs of 16-key tiles
     float c;             // scale * log2 e
 };
 
+// row r of a (batch, key head) is query r / G, head r % G of the key head's G
+HV_DEV void hv_cross_row(const HvCrossArgs& a, int r, int kvh, int& query, int& column) {
+    if (a.G == 1) {  // (uniform: spares the division)
+        query = r;
+        column = kvh * a.p.D;
+    } else {
+        query = r / a.G;
+        column = (kvh * a.G + (r - query * a.G)) * a.p.D;
+    }
+}
+
+// geometry of the LDS copies and of a lane's share of the output for head dim D
+template <int D>
+struct HvCrossGeom {
+    static constexpr int KS = (D + 31) / 32, DT = (D + 15) / 16, P8 = D / 8;
+    static constexpr int KSTR = KS * 64 + 16;                 // bytes of a K row: an odd number of 16-byte pieces (no bank conflicts)
+    static constexpr int VSTR = (DT % 2 ? DT : DT + 1) * 32;  // bytes of a V row: an odd number of 32-byte tiles (the transposed reads)
+    // output tiles come in pairs that share 32 columns: row 4 c + r of the first is column 8 c + r, of the second 8 c + 4 + r, so that a
+    // lane's eight values are neighbours (16-byte stores); an odd last tile is in order
+    static constexpr int PAIRED = DT / 2 * 2;
+    HV_DEV static int vbyte(int dt, int c) { return dt < PAIRED ? dt / 2 * 64 + c * 16 + (dt & 1) * 8 : dt * 32 + c * 8; }
+};
+
+// A operand of O^T = V^T P^T for output tile dt and the 32 keys from row0 on: lane t of a 16-lane group points at row t / 4, column
+// group t % 4 and receives column t of the 4 rows; the second read takes the 16-key tile behind
+template <int D>
+HV_DEV bf16x8 hv_cross_vfrag(const unsigned char* sV, int row0, int dt, int col, int g) {
+    using G = HvCrossGeom<D>;
+    const unsigned char* src = sV + (row0 + g * 4 + col / 4) * G::VSTR + G::vbyte(dt, col & 3);
+    const bf16x4 v0 = hv_lds_tr4(src), v1 = hv_lds_tr4(src + 16 * G::VSTR);
+    return bf16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+}
+
+// a row's D values of a head: o = acc / sum of weights, 0 where that is 0 (nothing attended)
+template <int D>
+HV_DEV void hv_cross_store(bf16_t* dst, const f32x4* acc, float sum, int g) {
+    using G = HvCrossGeom<D>;
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+    for (int d = 0; d < G::PAIRED; d += 2)
+        hv_st16(dst + d * 16 + g * 8, u32x4{hv_pack2(acc[d][0] * inv, acc[d][1] * inv), hv_pack2(acc[d][2] * inv, acc[d][3] * inv),
+                                            hv_pack2(acc[d + 1][0] * inv, acc[d + 1][1] * inv), hv_pack2(acc[d + 1][2] * inv, acc[d + 1][3] * inv)});
+    if constexpr (G::DT % 2 == 1) {
+        constexpr int d = G::DT - 1;
+        if (d * 16 + g * 4 < D) hv_st8(dst + d * 16 + g * 4, u32x2{hv_pack2(acc[d][0] * inv, acc[d][1] * inv), hv_pack2(acc[d][2] * inv, acc[d][3] * inv)});
+    }
+}
+
+HV_DEV bf16x8 hv_bf16_ones() { return bf16x8{0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80}; }
+
+// ---- few states (Lk <= 32 NP <= 96, D <= 80): a prompt.  The stream of queries is what counts -- q is read once, o written once, and
+// both products of 16 queries take less than the time their 4 KB spend on the bus.  All of K and V^T of a (batch, key head) stay in
+// a wave's REGISTERS as matrix operands (2 NP KS + NP DT fragments); after them a wave reads nothing but its next 16 queries, which
+// it requests one tile ahead, and meets no barrier.  No running maximum: a row's scores are all there.
+template <int D, int NP>
+__global__ __launch_bounds__(256, D == 40 ? 3 : 2) void hv_cross_attention_few_kernel(HvCrossArgs a) {
+    using G = HvCrossGeom<D>;
+    constexpr int KS = G::KS, DT = G::DT, P8 = G::P8, CH = 32 * NP;
+    __shared__ __attribute__((aligned(16))) unsigned char sK[CH * G::KSTR];
+    __shared__ __attribute__((aligned(16))) unsigned char sV[CH * G::VSTR];
+    __shared__ __attribute__((aligned(16))) float sBias[CH];
+    const int per_xcd = (a.units + 7) / 8;  // neighbouring units (the heads of one range of rows) on one XCD: they share cache lines
+    const int unit = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per_xcd || unit >= a.units) return;
+    const hv_cross_attention_params& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+    const int kvh = unit % p.kv_heads, group = unit / p.kv_heads % a.groups, b = unit / p.kv_heads / a.groups;
+    int len = p.kv_len ? p.kv_len[b] : p.Lk;
+    len = len < 0 ? 0 : len > p.Lk ? p.Lk : len;
+    const int nt = (len + 15) / 16;  // 16-key tiles with a state in reach
+    const u32x4 zero4 = {0u, 0u, 0u, 0u};
+    {
+        const bf16_t* Kb = p.K + (long)b * p.k_stride_b + (long)kvh * D;
+        const bf16_t* Vb = p.V + (long)b * p.v_stride_b + (long)kvh * D;
+        const uint8_t* mask = p.key_mask ? p.key_mask + (long)b * p.mask_stride_b : nullptr;
+        constexpr int KP = KS * 4, VP = DT * 2;  // pieces of a padded row
+        for (int i = tid; i < CH * KP; i += 256) {
+            const int row = i / KP, piece = i % KP;
+            const bool on = row < len && piece < P8 && (mask == nullptr || mask[row] != 0);
+            hv_st16(sK + row * G::KSTR + piece * 16, on ? hv_ld16(Kb + (long)row * p.ldk + piece * 8) : zero4);
+        }
+        for (int i = tid; i < CH * VP; i += 256) {
+            const int row = i / VP, piece = i % VP;
+            const bool on = row < len && piece < P8 && (mask == nullptr || mask[row] != 0);
+            hv_st16(sV + row * G::VSTR + piece * 16, on ? hv_ld16(Vb + (long)row * p.ldv + piece * 8) : zero4);
+        }
+        if (tid < CH) sBias[tid] = tid < len && (mask == nullptr || mask[tid] != 0) ? 0.f : -INFINITY;
+    }
+    __syncthreads();
+    bf16x8 kf[2 * NP][KS], vf[NP][DT];
+#pragma unroll
+    for (int kt = 0; kt < 2 * NP; ++kt)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) kf[kt][ks] = hv_as_bf16x8(hv_ld16(sK + (kt * 16 + col) * G::KSTR + ks * 64 + g * 16));
+#pragma unroll
+    for (int pr = 0; pr < NP; ++pr)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vf[pr][d] = hv_cross_vfrag<D>(sV, pr * 32, d, col, g);
+
+    const bf16_t* const Qb = p.Q + (long)b * p.q_stride_b;
+    bf16_t* const Ob = p.O + (long)b * p.o_stride_b;
+    const int end = min((group + 1) * a.per_wg, a.blocks);  // tiles of 16 rows
+    bf16x8 qf[KS];
+    auto load_q = [&](int tile) {
+        const int r = tile * 16 + col;
+        const bool on = tile < end && r < a.rows;
+        int query, column;
+        hv_cross_row(a, r, kvh, query, column);
+        const bf16_t* src = Qb + (long)query * p.ldq + column;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = hv_as_bf16x8(on && ks * 32 + g * 8 < D ? hv_ld16(src + ks * 32 + g * 8) : zero4);
+    };
+    int tile = group * a.per_wg + wave;
+    load_q(tile);
+    for (; tile < end; tile += 4) {
+        f32x4 s[2 * NP];
+        float top = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < 2 * NP; ++kt)
+            if (kt < nt) {
+                s[kt] = *reinterpret_cast<const f32x4*>(sBias + kt * 16 + g * 4);
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kt][ks], qf[ks], s[kt], 0, 0, 0);
+            }
+        load_q(tile + 4);  // in flight through the softmax and the second product
+#pragma unroll
+        for (int kt = 0; kt < 2 * NP; ++kt)
+            if (kt < nt) top = fmaxf(fmaxf(top, fmaxf(s[kt][0], s[kt][1])), fmaxf(s[kt][2], s[kt][3]));
+        top = hv_max_quarters(top);
+        const float mc = top == -INFINITY ? 0.f : -top * a.c;  // nothing attended: 2^(-inf - 0) = 0
+        f32x4 acc[DT], sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int pr = 0; pr < NP; ++pr)
+            if (2 * pr < nt) {
+                u32x4 w = zero4;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (2 * pr + h < nt) {
+                        float f[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) f[e] = __builtin_amdgcn_exp2f(fmaf(s[2 * pr + h][e], a.c, mc));
+                        w[2 * h] = hv_pack2(f[0], f[1]);
+                        w[2 * h + 1] = hv_pack2(f[2], f[3]);
+                    }
+                const bf16x8 pf = hv_as_bf16x8(w);
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_bf16_ones(), pf, sum, 0, 0, 0);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[pr][d], pf, acc[d], 0, 0, 0);
+            }
+        const int r = tile * 16 + col;
+        int query, column;
+        hv_cross_row(a, r, kvh, query, column);
+        if (r < a.rows) hv_cross_store<D>(Ob + (long)query * p.ldo + column, acc, sum[0], g);
+    }
+}
+
 template <int D, int QT, int NP>
-__global__ __launch_bounds__(256) void hv_cross_attention_kernel(HvCrossArgs a) {
-    constexpr int KS = (D + 31) / 32, DT = (D + 15) / 16, P8 = D / 8, CH = 32 * NP;
-    constexpr int KSTR = KS * 64 + 16;                     // bytes of a K row: an odd number of 16-byte pieces (no bank conflicts)
-    constexpr int VSTR = (DT % 2 ? DT : DT + 1) * 32;      // bytes of a V row: an odd number of 32-byte tiles (the transposed reads)
+__global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_attention_kernel(HvCrossArgs a) {
+    using Geom = HvCrossGeom<D>;
+    constexpr int KS = Geom::KS, DT = Geom::DT, P8 = Geom::P8, CH = 32 * NP, KSTR = Geom::KSTR, VSTR = Geom::VSTR;
     constexpr int NV = (CH * P8 + 255) / 256;              // 16-byte pieces of K (and of V) that a thread stages
     __shared__ __attribute__((aligned(16))) unsigned char sK[CH * KSTR];
     __shared__ __attribute__((aligned(16))) unsigned char sV[CH * VSTR];
@@ -121,20 +279,16 @@ __global__ __launch_bounds__(256) void hv_cross_attention_kernel(HvCrossArgs a) 
         }
         if (tid < CH) sBias[tid] = breg;
     };
-    if (chunks == 1) {  // the states fit one chunk: they stay in LDS for all row blocks
-        fetch(k_begin);
-        stage();
-        __syncthreads();
-    }
-
-    const int blk_end = min((group + 1) * a.per_wg, a.blocks);
-    for (int blk = group * a.per_wg; blk < blk_end; ++blk) {
-        const int r0 = (blk * 4 + wave) * QT * 16 + col;
+    fetch(k_begin);
+    {
+        const int r0 = (group * 4 + wave) * QT * 16 + col;
         bf16x8 qf[QT][KS];
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             const int r = r0 + t * 16;
-            const bf16_t* src = p.Q + (long)b * p.q_stride_b + (long)(r / a.G) * p.ldq + (long)(kvh * a.G + r % a.G) * D;
+            int query, column;
+            hv_cross_row(a, r, kvh, query, column);
+            const bf16_t* src = p.Q + (long)b * p.q_stride_b + (long)query * p.ldq + column;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
                 qf[t][ks] = hv_as_bf16x8(r < a.rows && ks * 32 + g * 8 < D ? hv_ld16(src + ks * 32 + g * 8) : zero4);
@@ -148,15 +302,12 @@ __global__ __launch_bounds__(256) void hv_cross_attention_kernel(HvCrossArgs a) 
 #pragma unroll
             for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        if (chunks > 1) fetch(k_begin);
         for (int ch = 0; ch < chunks; ++ch) {
             const int n = k_end - k_begin - ch * CH;  // keys left
-            if (chunks > 1) {
-                __syncthreads();  // the readers of the previous chunk are done
-                stage();
-                __syncthreads();
-                if (ch + 1 < chunks) fetch(k_begin + (ch + 1) * CH);
-            }
+            if (ch > 0) __syncthreads();  // the readers of the previous chunk are done
+            stage();
+            __syncthreads();
+            if (ch + 1 < chunks) fetch(k_begin + (ch + 1) * CH);
             f32x4 s[QT][2 * NP];
             float top[QT];
 #pragma unroll
@@ -204,15 +355,11 @@ __global__ __launch_bounds__(256) void hv_cross_attention_kernel(HvCrossArgs a) 
                         for (int e = 0; e < 8; ++e) f[e] = __builtin_amdgcn_exp2f(fmaf(s[t][2 * pr + e / 4][e % 4], a.c, mc[t]));
                         pf[t] = hv_as_bf16x8(hv_pack8(f));
                     }
-                    const bf16x8 ones = {0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80};
 #pragma unroll
-                    for (int t = 0; t < QT; ++t) lsum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[t], lsum[t], 0, 0, 0);
+                    for (int t = 0; t < QT; ++t) lsum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_bf16_ones(), pf[t], lsum[t], 0, 0, 0);
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
-                        // lane t of a 16-lane group points at row t / 4, columns 4 (t % 4) and receives column t of the 4 rows
-                        const unsigned char* src = sV + (pr * 32 + g * 4 + col / 4) * VSTR + d * 32 + (col & 3) * 8;
-                        const bf16x4 v0 = hv_lds_tr4(src), v1 = hv_lds_tr4(src + 16 * VSTR);
-                        const bf16x8 vf = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                        const bf16x8 vf = hv_cross_vfrag<D>(sV, pr * 32, d, col, g);
 #pragma unroll
                         for (int t = 0; t < QT; ++t) acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], acc[t][d], 0, 0, 0);
                     }
@@ -226,24 +373,21 @@ __global__ __launch_bounds__(256) void hv_cross_attention_kernel(HvCrossArgs a) 
             if (a.splits > 1) {  // unnormalised sums, with the maximum and the sum of weights they refer to
                 float* dst = p.workspace + ((((long)b * p.kv_heads + kvh) * a.rows + r) * a.splits + split) * (D + 2);
 #pragma unroll
-                for (int d = 0; d < DT; ++d)
-                    if (d * 16 + g * 4 < D) {
+                for (int d = 0; d < DT; ++d) {
+                    const int at = d < Geom::PAIRED ? d / 2 * 32 + g * 8 + (d & 1) * 4 : d * 16 + g * 4;
+                    if (at < D) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) dst[2 + d * 16 + g * 4 + e] = acc[t][d][e];
+                        for (int e = 0; e < 4; ++e) dst[2 + at + e] = acc[t][d][e];
                     }
+                }
                 if (g == 0) {
                     dst[0] = m[t];
                     dst[1] = lsum[t][0];
                 }
             } else {
-                const float inv = lsum[t][0] == 0.f ? 0.f : 1.0f / lsum[t][0];
-                bf16_t* dst = p.O + (long)b * p.o_stride_b + (long)(r / a.G) * p.ldo + (long)(kvh * a.G + r % a.G) * D;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-                    if (d * 16 + g * 4 < D) {
-                        const u32x2 w = {hv_pack2(acc[t][d][0] * inv, acc[t][d][1] * inv), hv_pack2(acc[t][d][2] * inv, acc[t][d][3] * inv)};
-                        hv_st8(dst + d * 16 + g * 4, w);
-                    }
+                int query, column;
+                hv_cross_row(a, r, kvh, query, column);
+                hv_cross_store<D>(p.O + (long)b * p.o_stride_b + (long)query * p.ldo + column, acc[t], lsum[t][0], g);
             }
         }
     }
@@ -274,38 +418,51 @@ __global__ __launch_bounds__(256) void hv_cross_attention_join_kernel(HvCrossArg
             if (i * 64 + lane < D) o[i] += w * q[2 + i * 64 + lane];
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
-    bf16_t* dst = p.O + (long)b * p.o_stride_b + (long)(r / a.G) * p.ldo + (long)(kvh * a.G + r % a.G) * D;
+    int query, column;
+    hv_cross_row(a, r, kvh, query, column);
+    bf16_t* dst = p.O + (long)b * p.o_stride_b + (long)query * p.ldo + column;
 #pragma unroll
     for (int i = 0; i < (D + 63) / 64; ++i)
         if (i * 64 + lane < D) dst[i * 64 + lane] = hv_f2bf(o[i] * inv);
 }
 
 // sizes -> how the work is cut (also what hv_cross_attention_workspace answers from): -1 invalid, -2 head dim
-static inline int hv_cross_attention_plan(const hv_cross_attention_params& p, HvCrossArgs& a, int& qt, int& np) {
+static inline int hv_cross_attention_plan(const hv_cross_attention_params& p, HvCrossArgs& a) {
     if (p.B < 0 || p.Lq < 0 || p.Lk < 0 || p.heads <= 0 || p.kv_heads <= 0 || p.heads % p.kv_heads != 0) return -1;
     if (p.D != 40 && p.D != 64 && p.D != 80 && p.D != 128 && p.D != 160) return -2;
-    const long rows = (long)p.Lq * (p.heads / p.kv_heads);
-    if (rows > 0x3fffffffL) return -1;
+    const long rows = (long)p.Lq * (p.heads / p.kv_heads), pairs = (long)p.B * p.kv_heads;
+    if (rows > 0x3fffffffL || pairs > 0x3fffffffL) return -1;
     a.p = p;
     a.G = p.heads / p.kv_heads;
     a.rows = (int)rows;
-    qt = rows > 64 ? 2 : 1;
-    np = p.Lk > 64 && p.Lk <= 96 ? 3 : 2;
-    a.blocks = (int)((rows + 64 * qt - 1) / (64 * qt));
-    const long base = (long)p.B * p.kv_heads * a.blocks;
     a.splits = 1;
-    if (base < 512 && p.Lk >= 256) {  // too few workgroups to fill the chip: cut the keys
-        const long want = (1024 + base - 1) / (base > 0 ? base : 1), most = p.Lk / 128;
-        a.splits = (int)(want < most ? want : most);
-        if (a.splits < 1) a.splits = 1;
+    a.c = p.scale * 1.44269504088896341f;
+    long units;
+    a.few = p.Lk <= 96 && p.D <= 80;
+    if (a.few) {  // tiles of 16 rows, ranges of them for about four rounds of the workgroups that fit the chip
+        a.np = p.Lk <= 32 ? 1 : p.Lk <= 64 ? 2 : 3;
+        a.qt = 1;
+        a.blocks = (int)((rows + 15) / 16);
+        const long fit = 256L * (p.D == 40 ? 3 : 2), groups = (fit * 4 + pairs - 1) / (pairs > 0 ? pairs : 1);
+        a.per_wg = (int)((a.blocks + groups - 1) / groups);
+        a.per_wg = (a.per_wg + 3) / 4 * 4;
+        if (a.per_wg < 4) a.per_wg = 4;
+    } else {
+        a.qt = rows > 64 ? 2 : 1;
+        a.np = 2;
+        a.blocks = (int)((rows + 64 * a.qt - 1) / (64 * a.qt));
+        a.per_wg = 1;
+        const long base = pairs * a.blocks;
+        if (base < 512 && p.Lk >= 256) {  // too few workgroups to fill the chip: cut the keys
+            const long want = (1024 + base - 1) / (base > 0 ? base : 1), most = p.Lk / 128;
+            a.splits = (int)(want < most ? want : most);
+            if (a.splits < 1) a.splits = 1;
+        }
     }
-    a.per_wg = 1;
-    if (p.Lk <= 32 * np) a.per_wg = (int)(base / 4096 < 1 ? 1 : base / 4096 > 16 ? 16 : base / 4096);
     a.groups = (a.blocks + a.per_wg - 1) / a.per_wg;
-    const long units = (long)p.B * p.kv_heads * a.groups * a.splits;
+    units = pairs * a.groups * a.splits;
     if (units > 0x3fffffffL) return -1;
     a.units = (int)units;
-    a.c = p.scale * 1.44269504088896341f;
     return 0;
 }
 
@@ -314,13 +471,20 @@ static inline long hv_cross_attention_floats(const HvCrossArgs& a) {
 }
 
 template <int D>
-static inline void hv_cross_attention_launch_d(const HvCrossArgs& a, int qt, int np, hipStream_t stream) {
+static inline void hv_cross_attention_launch_d(const HvCrossArgs& a, hipStream_t stream) {
     const dim3 grid((unsigned)((a.units + 7) / 8 * 8)), block(256);
-    hv_note("hv_cross_attention_kernel<%d,%d,%d> | B=%d Lq=%d Lk=%d heads=%d/%d splits=%d", D, qt, np, a.p.B, a.p.Lq, a.p.Lk, a.p.heads,
+    if constexpr (D <= 80) {
+        if (a.few) {
+            hv_note("hv_cross_attention_few_kernel<%d,%d> | B=%d Lq=%d Lk=%d heads=%d/%d", D, a.np, a.p.B, a.p.Lq, a.p.Lk, a.p.heads, a.p.kv_heads);
+            if (a.np == 1) hv_launch(hv_cross_attention_few_kernel<D, 1>, grid, block, stream, a);
+            else if (a.np == 2) hv_launch(hv_cross_attention_few_kernel<D, 2>, grid, block, stream, a);
+            else hv_launch(hv_cross_attention_few_kernel<D, 3>, grid, block, stream, a);
+            return;
+        }
+    }
+    hv_note("hv_cross_attention_kernel<%d,%d> | B=%d Lq=%d Lk=%d heads=%d/%d splits=%d", D, a.qt, a.p.B, a.p.Lq, a.p.Lk, a.p.heads,
             a.p.kv_heads, a.splits);
-    if (qt == 2 && np == 3) hv_launch(hv_cross_attention_kernel<D, 2, 3>, grid, block, stream, a);
-    else if (qt == 2) hv_launch(hv_cross_attention_kernel<D, 2, 2>, grid, block, stream, a);
-    else if (np == 3) hv_launch(hv_cross_attention_kernel<D, 1, 3>, grid, block, stream, a);
+    if (a.qt == 2) hv_launch(hv_cross_attention_kernel<D, 2, 2>, grid, block, stream, a);
     else hv_launch(hv_cross_attention_kernel<D, 1, 2>, grid, block, stream, a);
     if (a.splits > 1) {
         const long items = (long)a.p.B * a.p.kv_heads * a.rows;
@@ -331,15 +495,13 @@ static inline void hv_cross_attention_launch_d(const HvCrossArgs& a, int qt, int
 
 static inline long hv_cross_attention_workspace_of(const hv_cross_attention_params& p) {
     HvCrossArgs a;
-    int qt, np;
-    const int rc = hv_cross_attention_plan(p, a, qt, np);
+    const int rc = hv_cross_attention_plan(p, a);
     return rc ? rc : hv_cross_attention_floats(a);
 }
 
 static inline int hv_cross_attention_launch(const hv_cross_attention_params& p, hipStream_t stream) {
     HvCrossArgs a;
-    int qt, np;
-    const int rc = hv_cross_attention_plan(p, a, qt, np);
+    const int rc = hv_cross_attention_plan(p, a);
     if (rc) return rc;
     if (!(p.scale > 0.f) || p.scale > 3.0e38f) return -1;
     if (p.B == 0 || p.Lq == 0) return 0;
@@ -348,11 +510,11 @@ static inline int hv_cross_attention_launch(const hv_cross_attention_params& p, 
     if ((addr & 15) != 0 || (strides & 7) != 0) return -1;
     if (hv_cross_attention_floats(a) > p.workspace_floats || (a.splits > 1 && (p.workspace == nullptr || ((uint64_t)p.workspace & 3) != 0))) return -3;
     switch (p.D) {
-        case 40: hv_cross_attention_launch_d<40>(a, qt, np, stream); break;
-        case 64: hv_cross_attention_launch_d<64>(a, qt, np, stream); break;
-        case 80: hv_cross_attention_launch_d<80>(a, qt, np, stream); break;
-        case 128: hv_cross_attention_launch_d<128>(a, qt, np, stream); break;
-        default: hv_cross_attention_launch_d<160>(a, qt, np, stream); break;
+        case 40: hv_cross_attention_launch_d<40>(a, stream); break;
+        case 64: hv_cross_attention_launch_d<64>(a, stream); break;
+        case 80: hv_cross_attention_launch_d<80>(a, stream); break;
+        case 128: hv_cross_attention_launch_d<128>(a, stream); break;
+        default: hv_cross_attention_launch_d<160>(a, stream); break;
     }
     return 0;
 }
