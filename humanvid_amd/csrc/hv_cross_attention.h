@@ -47,9 +47,11 @@ struct HvCrossArgs {
     int groups;          // ceil(blocks / per_wg)
     int units;           // workgroups with work
     int splits;          // ranges the keys are cut into
-    int few, qt, np;     // which kernel; 16-row tiles per wave; pairs of 16-key tiles
+    int few, qt;         // which kernel; its 16-row tiles per wave
     float c;             // scale * log2 e
 };
+
+#define HV_CROSS_FEW_ROWS(D) ((D) == 40 ? 64 : 32)  // hv_cross_attention_few_kernel: rows whose pieces fill whole copy instructions
 
 // row r of a (batch, key head) is query r / G, head r % G of the key head's G
 HV_DEV void hv_cross_row(const HvCrossArgs& a, int r, int kvh, int& query, int& column) {
@@ -84,44 +86,67 @@ HV_DEV bf16x8 hv_cross_vfrag(const unsigned char* sV, int row0, int dt, int col,
     return bf16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
 }
 
-// a row's D values of a head: o = acc / sum of weights, 0 where that is 0 (nothing attended)
-template <int D>
-HV_DEV void hv_cross_store(bf16_t* dst, const f32x4* acc, float sum, int g) {
+// a row's D values of a head: o = acc / sum of weights, 0 where that is 0 (nothing attended); at(piece) is where its 16-byte piece lies
+template <int D, class At>
+HV_DEV void hv_cross_store(At at, const f32x4* acc, float sum, int g) {
     using G = HvCrossGeom<D>;
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const float inv = sum == 0.f ? 0.f : __builtin_amdgcn_rcpf(sum);  // (within 2^-23: the output keeps 2^-8)
 #pragma unroll
     for (int d = 0; d < G::PAIRED; d += 2)
-        hv_st16(dst + d * 16 + g * 8, u32x4{hv_pack2(acc[d][0] * inv, acc[d][1] * inv), hv_pack2(acc[d][2] * inv, acc[d][3] * inv),
-                                            hv_pack2(acc[d + 1][0] * inv, acc[d + 1][1] * inv), hv_pack2(acc[d + 1][2] * inv, acc[d + 1][3] * inv)});
+        hv_st16(at(d * 2 + g), u32x4{hv_pack2(acc[d][0] * inv, acc[d][1] * inv), hv_pack2(acc[d][2] * inv, acc[d][3] * inv),
+                                     hv_pack2(acc[d + 1][0] * inv, acc[d + 1][1] * inv), hv_pack2(acc[d + 1][2] * inv, acc[d + 1][3] * inv)});
     if constexpr (G::DT % 2 == 1) {
         constexpr int d = G::DT - 1;
-        if (d * 16 + g * 4 < D) hv_st8(dst + d * 16 + g * 4, u32x2{hv_pack2(acc[d][0] * inv, acc[d][1] * inv), hv_pack2(acc[d][2] * inv, acc[d][3] * inv)});
+        if (d * 16 + g * 4 < D)
+            hv_st8((char*)at(d * 2 + g / 2) + (g & 1) * 8, u32x2{hv_pack2(acc[d][0] * inv, acc[d][1] * inv), hv_pack2(acc[d][2] * inv, acc[d][3] * inv)});
     }
+}
+
+// between a wave's own LDS writes and other lanes' reads of them: the LDS serves a wave in order, the compiler has to keep that order
+HV_DEV void hv_wave_fence() {
+#ifndef HV_EMU
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+#else
+    (void)__shfl_xor(0, 1);  // the emulator runs lanes one after the other up to the next collective
+#endif
 }
 
 HV_DEV bf16x8 hv_bf16_ones() { return bf16x8{0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80}; }
 
-// ---- few states (Lk <= 32 NP <= 96, D <= 80): a prompt.  The stream of queries is what counts -- q is read once, o written once, and
-// both products of 16 queries take less than the time their 4 KB spend on the bus.  All of K and V^T of a (batch, key head) stay in
-// a wave's REGISTERS as matrix operands (2 NP KS + NP DT fragments); after them a wave reads nothing but its next 16 queries, which
-// it requests one tile ahead, and meets no barrier.  No running maximum: a row's scores are all there.
-template <int D, int NP>
+// ---- few states (Lk <= 16 NT <= 96, D <= 80): a prompt.  The stream of queries is what counts -- q is read once, o written once.
+// All of K and V^T of a (batch, key head) stay in a wave's REGISTERS as matrix operands.  A wave then streams tiles of ROWS queries
+// through two LDS slots of its own: the next tile is in flight by LDS-DMA while this one is computed, the results replace the
+// queries in the slot and leave it row by row.  (Straight from memory into operand registers the 16 lanes of an access lie in 16
+// rows -- 16 cache lines for 256 bytes: 133 us instead of XX at 2 x 147456 queries, 77 states, D = 40.)  A wave meets no barrier after the
+// states are loaded.  No running maximum: a row's scores are all there.  The number of 16-key tiles is a template argument:
+// branches around absent tiles cost more than a masked tile (twice the instructions).  G divides 32, so a lane's offsets inside a
+// tile are the same for every tile.
+template <int D, int NT>
 __global__ __launch_bounds__(256, D == 40 ? 3 : 2) void hv_cross_attention_few_kernel(HvCrossArgs a) {
     using G = HvCrossGeom<D>;
-    constexpr int KS = G::KS, DT = G::DT, P8 = G::P8, CH = 32 * NP;
-    __shared__ __attribute__((aligned(16))) unsigned char sK[CH * G::KSTR];
-    __shared__ __attribute__((aligned(16))) unsigned char sV[CH * G::VSTR];
+    constexpr int KS = G::KS, DT = G::DT, P8 = G::P8, NP = (NT + 1) / 2, CH = 32 * NP;
+    constexpr int ROWS = HV_CROSS_FEW_ROWS(D), NI = ROWS * P8 / 64, SLOT = ROWS * D * 2;
+    static_assert(ROWS * P8 % 64 == 0, "whole copy instructions");
+    constexpr int STATES = CH * (G::KSTR + G::VSTR), SMEM = STATES > 8 * SLOT ? STATES : 8 * SLOT;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[SMEM];  // first the states, then 4 waves x 2 slots
     __shared__ __attribute__((aligned(16))) float sBias[CH];
     const int per_xcd = (a.units + 7) / 8;  // neighbouring units (the heads of one range of rows) on one XCD: they share cache lines
     const int unit = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per_xcd || unit >= a.units) return;
     const hv_cross_attention_params& p = a.p;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+#ifndef HV_EMU
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#else
+    const int wave = tid >> 6;
+#endif
     const int kvh = unit % p.kv_heads, group = unit / p.kv_heads % a.groups, b = unit / p.kv_heads / a.groups;
     int len = p.kv_len ? p.kv_len[b] : p.Lk;
     len = len < 0 ? 0 : len > p.Lk ? p.Lk : len;
-    const int nt = (len + 15) / 16;  // 16-key tiles with a state in reach
     const u32x4 zero4 = {0u, 0u, 0u, 0u};
+    unsigned char* const sK = smem;
+    unsigned char* const sV = smem + CH * G::KSTR;
     {
         const bf16_t* Kb = p.K + (long)b * p.k_stride_b + (long)kvh * D;
         const bf16_t* Vb = p.V + (long)b * p.v_stride_b + (long)kvh * D;
@@ -140,57 +165,82 @@ __global__ __launch_bounds__(256, D == 40 ? 3 : 2) void hv_cross_attention_few_k
         if (tid < CH) sBias[tid] = tid < len && (mask == nullptr || mask[tid] != 0) ? 0.f : -INFINITY;
     }
     __syncthreads();
-    bf16x8 kf[2 * NP][KS], vf[NP][DT];
+    bf16x8 kf[NT][KS], vf[NP][DT];
 #pragma unroll
-    for (int kt = 0; kt < 2 * NP; ++kt)
+    for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) kf[kt][ks] = hv_as_bf16x8(hv_ld16(sK + (kt * 16 + col) * G::KSTR + ks * 64 + g * 16));
 #pragma unroll
     for (int pr = 0; pr < NP; ++pr)
 #pragma unroll
         for (int d = 0; d < DT; ++d) vf[pr][d] = hv_cross_vfrag<D>(sV, pr * 32, d, col, g);
+    __syncthreads();  // every wave has its operands: the slots may be written
 
-    const bf16_t* const Qb = p.Q + (long)b * p.q_stride_b;
-    bf16_t* const Ob = p.O + (long)b * p.o_stride_b;
-    const int end = min((group + 1) * a.per_wg, a.blocks);  // tiles of 16 rows
-    bf16x8 qf[KS];
-    auto load_q = [&](int tile) {
-        const int r = tile * 16 + col;
-        const bool on = tile < end && r < a.rows;
-        int query, column;
-        hv_cross_row(a, r, kvh, query, column);
-        const bf16_t* src = Qb + (long)query * p.ldq + column;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) qf[ks] = hv_as_bf16x8(on && ks * 32 + g * 8 < D ? hv_ld16(src + ks * 32 + g * 8) : zero4);
+    // slot layout: row major, 16-byte pieces; rows of 128 bytes (D = 64) with their pieces XOR-swizzled, as their fragment reads would
+    // all start in the same banks (rows of 80 and 160 bytes do not)
+    auto slot_of = [](int row, int piece) { return (row * P8 + (D == 64 ? piece ^ (row & 7) : piece)) * 16; };
+    const int end = min((group + 1) * a.per_wg, a.blocks);  // tiles of ROWS rows
+    const bf16_t* const Qb = p.Q + (long)b * p.q_stride_b + (long)kvh * a.G * D;
+    bf16_t* const Ob = p.O + (long)b * p.o_stride_b + (long)kvh * a.G * D;
+    auto offset = [&](int i, int last, long ld) {  // byte offset inside a tile of the piece that lane and instruction i carry
+        const int idx = i * 64 + lane, slot = idx % P8;
+        int row = idx / P8;
+        const int piece = D == 64 ? slot ^ (row & 7) : slot;
+        row = min(row, last);
+        const int query = a.G == 1 ? row : row / a.G;
+        return (unsigned)query * (unsigned)(ld * 2) + (unsigned)((row - query * a.G) * D * 2 + piece * 16);
     };
+    unsigned qofs[NI], oofs[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        qofs[i] = offset(i, ROWS, p.ldq);
+        oofs[i] = offset(i, ROWS, p.ldo);
+    }
+    auto issue = [&](int tile, unsigned char* slot) {
+        const char* base = (const char*)(Qb + (long)(tile * ROWS / a.G) * p.ldq);
+        const int last = a.rows - 1 - tile * ROWS;
+        if (last >= ROWS - 1) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) hv_glds16_s(base, qofs[i], slot + i * 1024);
+        } else {  // rows behind the last repeat it and are not stored
+#pragma unroll
+            for (int i = 0; i < NI; ++i) hv_glds16_s(base, offset(i, last, p.ldq), slot + i * 1024);
+        }
+    };
+    unsigned char* slot = smem + wave * 2 * SLOT;
+    unsigned char* other = slot + SLOT;
     int tile = group * a.per_wg + wave;
-    load_q(tile);
-    for (; tile < end; tile += 4) {
-        f32x4 s[2 * NP];
-        float top = -INFINITY;
+    if (tile < end) issue(tile, slot);
+    for (bool first = true; tile < end; tile += 4, first = false) {
+        // in flight, in order: this tile's copies, the stores of the tile before (all NI of them: it was not the last)
+        if (first) hv_vm_wait<0>();
+        else hv_vm_wait<NI>();
+        hv_wave_fence();
+        if (tile + 4 < end) issue(tile + 4, other);
+#pragma unroll 1
+        for (int sub = 0; sub < ROWS; sub += 16) {
+            f32x4 s[NT];
 #pragma unroll
-        for (int kt = 0; kt < 2 * NP; ++kt)
-            if (kt < nt) {
-                s[kt] = *reinterpret_cast<const f32x4*>(sBias + kt * 16 + g * 4);
+            for (int kt = 0; kt < NT; ++kt) s[kt] = *reinterpret_cast<const f32x4*>(sBias + kt * 16 + g * 4);
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kt][ks], qf[ks], s[kt], 0, 0, 0);
+            for (int ks = 0; ks < KS; ++ks) {
+                u32x4 q = zero4;
+                if ((ks + 1) * 32 <= D || ks * 32 + g * 8 < D) q = hv_ld16(slot + slot_of(sub + col, ks * 4 + g));
+#pragma unroll
+                for (int kt = 0; kt < NT; ++kt) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kt][ks], hv_as_bf16x8(q), s[kt], 0, 0, 0);
             }
-        load_q(tile + 4);  // in flight through the softmax and the second product
+            float top = -INFINITY;
 #pragma unroll
-        for (int kt = 0; kt < 2 * NP; ++kt)
-            if (kt < nt) top = fmaxf(fmaxf(top, fmaxf(s[kt][0], s[kt][1])), fmaxf(s[kt][2], s[kt][3]));
-        top = hv_max_quarters(top);
-        const float mc = top == -INFINITY ? 0.f : -top * a.c;  // nothing attended: 2^(-inf - 0) = 0
-        f32x4 acc[DT], sum = {0.f, 0.f, 0.f, 0.f};
+            for (int kt = 0; kt < NT; ++kt) top = fmaxf(fmaxf(top, fmaxf(s[kt][0], s[kt][1])), fmaxf(s[kt][2], s[kt][3]));
+            top = hv_max_quarters(top);
+            const float mc = top == -INFINITY ? 0.f : -top * a.c;  // nothing attended: 2^(-inf - 0) = 0
+            f32x4 acc[DT], sum;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int pr = 0; pr < NP; ++pr)
-            if (2 * pr < nt) {
+            for (int pr = 0; pr < NP; ++pr) {
                 u32x4 w = zero4;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    if (2 * pr + h < nt) {
+                    if (2 * pr + h < NT) {
                         float f[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) f[e] = __builtin_amdgcn_exp2f(fmaf(s[2 * pr + h][e], a.c, mc));
@@ -198,14 +248,26 @@ __global__ __launch_bounds__(256, D == 40 ? 3 : 2) void hv_cross_attention_few_k
                         w[2 * h + 1] = hv_pack2(f[2], f[3]);
                     }
                 const bf16x8 pf = hv_as_bf16x8(w);
-                sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_bf16_ones(), pf, sum, 0, 0, 0);
+                const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_bf16_ones(), pf, pr ? sum : none, 0, 0, 0);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[pr][d], pf, acc[d], 0, 0, 0);
+                for (int d = 0; d < DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[pr][d], pf, pr ? acc[d] : none, 0, 0, 0);
             }
-        const int r = tile * 16 + col;
-        int query, column;
-        hv_cross_row(a, r, kvh, query, column);
-        if (r < a.rows) hv_cross_store<D>(Ob + (long)query * p.ldo + column, acc, sum[0], g);
+            hv_wave_fence();
+            hv_cross_store<D>([&](int piece) { return slot + slot_of(sub + col, piece); }, acc, sum[0], g);
+        }
+        hv_wave_fence();
+        char* base = (char*)(Ob + (long)(tile * ROWS / a.G) * p.ldo);
+        u32x4 out[NI];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) out[i] = hv_ld16(slot + i * 1024 + lane * 16);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            if (tile * ROWS + (i * 64 + lane) / P8 < a.rows) hv_st16(base + oofs[i], out[i]);
+        hv_wave_fence();  // (the stores wait for their data: the slot is free when they are issued)
+        unsigned char* const t = slot;
+        slot = other;
+        other = t;
     }
 }
 
@@ -387,7 +449,8 @@ __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_atte
             } else {
                 int query, column;
                 hv_cross_row(a, r, kvh, query, column);
-                hv_cross_store<D>(p.O + (long)b * p.o_stride_b + (long)query * p.ldo + column, acc[t], lsum[t][0], g);
+                bf16_t* dst = p.O + (long)b * p.o_stride_b + (long)query * p.ldo + column;
+                hv_cross_store<D>([&](int piece) { return dst + piece * 8; }, acc[t], lsum[t][0], g);
             }
         }
     }
@@ -438,18 +501,16 @@ static inline int hv_cross_attention_plan(const hv_cross_attention_params& p, Hv
     a.splits = 1;
     a.c = p.scale * 1.44269504088896341f;
     long units;
-    a.few = p.Lk <= 96 && p.D <= 80;
-    if (a.few) {  // tiles of 16 rows, ranges of them for about four rounds of the workgroups that fit the chip
-        a.np = p.Lk <= 32 ? 1 : p.Lk <= 64 ? 2 : 3;
-        a.qt = 1;
-        a.blocks = (int)((rows + 15) / 16);
+    a.few = p.Lk <= 96 && p.D <= 80 && 32 % a.G == 0 && p.ldq < (1L << 24) && p.ldo < (1L << 24);
+    if (a.few) {  // ranges of tiles for about four rounds of the workgroups that fit the chip
+        const int tile = HV_CROSS_FEW_ROWS(p.D);
+        a.blocks = (int)((rows + tile - 1) / tile);
         const long fit = 256L * (p.D == 40 ? 3 : 2), groups = (fit * 4 + pairs - 1) / (pairs > 0 ? pairs : 1);
         a.per_wg = (int)((a.blocks + groups - 1) / groups);
         a.per_wg = (a.per_wg + 3) / 4 * 4;
         if (a.per_wg < 4) a.per_wg = 4;
     } else {
         a.qt = rows > 64 ? 2 : 1;
-        a.np = 2;
         a.blocks = (int)((rows + 64 * a.qt - 1) / (64 * a.qt));
         a.per_wg = 1;
         const long base = pairs * a.blocks;
@@ -475,10 +536,12 @@ static inline void hv_cross_attention_launch_d(const HvCrossArgs& a, hipStream_t
     const dim3 grid((unsigned)((a.units + 7) / 8 * 8)), block(256);
     if constexpr (D <= 80) {
         if (a.few) {
-            hv_note("hv_cross_attention_few_kernel<%d,%d> | B=%d Lq=%d Lk=%d heads=%d/%d", D, a.np, a.p.B, a.p.Lq, a.p.Lk, a.p.heads, a.p.kv_heads);
-            if (a.np == 1) hv_launch(hv_cross_attention_few_kernel<D, 1>, grid, block, stream, a);
-            else if (a.np == 2) hv_launch(hv_cross_attention_few_kernel<D, 2>, grid, block, stream, a);
-            else hv_launch(hv_cross_attention_few_kernel<D, 3>, grid, block, stream, a);
+            const int nt = a.p.Lk <= 32 ? 2 : a.p.Lk <= 64 ? 4 : a.p.Lk <= 80 ? 5 : 6;
+            hv_note("hv_cross_attention_few_kernel<%d,%d> | B=%d Lq=%d Lk=%d heads=%d/%d", D, nt, a.p.B, a.p.Lq, a.p.Lk, a.p.heads, a.p.kv_heads);
+            if (nt == 2) hv_launch(hv_cross_attention_few_kernel<D, 2>, grid, block, stream, a);
+            else if (nt == 4) hv_launch(hv_cross_attention_few_kernel<D, 4>, grid, block, stream, a);
+            else if (nt == 5) hv_launch(hv_cross_attention_few_kernel<D, 5>, grid, block, stream, a);
+            else hv_launch(hv_cross_attention_few_kernel<D, 6>, grid, block, stream, a);
             return;
         }
     }
