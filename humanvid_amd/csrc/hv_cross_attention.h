@@ -20,6 +20,10 @@
 #include "hv_common.h"
 #include "humanvid_hip.h"
 
+// a NaN wins (v_maximum3_f32: no quieting of the operands first, as fmaxf would have it): its row is NaN either way
+HV_DEV float hv_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+HV_DEV float hv_max5(float m, const f32x4& s) { return hv_max(hv_max(hv_max(hv_max(m, s[0]), s[1]), s[2]), s[3]); }
+
 #ifndef HV_EMU
 // max over the four lanes with equal lane & 15
 HV_DEV float hv_max_quarters(float x) {
@@ -27,16 +31,16 @@ HV_DEV float hv_max_quarters(float x) {
     unsigned u = __builtin_bit_cast(unsigned, x);
     const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // a[0]: the lower half's values in both halves, a[1]: the upper's
     unsigned lo = a[0], hi = a[1];
-    x = fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+    x = hv_max(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
     u = __builtin_bit_cast(unsigned, x);
     const auto b = __builtin_amdgcn_permlane16_swap(u, u, false, false);  // the same for the two 16-lane rows of a half
     lo = b[0], hi = b[1];
-    return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+    return hv_max(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
 }
 #else
 HV_DEV float hv_max_quarters(float x) {
-    x = fmaxf(x, __shfl_xor(x, 32));
-    return fmaxf(x, __shfl_xor(x, 16));
+    x = hv_max(x, __shfl_xor(x, 32));
+    return hv_max(x, __shfl_xor(x, 16));
 }
 #endif
 
@@ -51,7 +55,7 @@ struct HvCrossArgs {
     float c;             // scale * log2 e
 };
 
-#define HV_CROSS_FEW_ROWS(D) ((D) == 40 ? 64 : 32)  // hv_cross_attention_few_kernel: rows whose pieces fill whole copy instructions
+#define HV_CROSS_FEW_ROWS(D) ((D) == 40 ? 64 : 32)  // hv_cross_attention_few_kernel: queries whose pieces fill whole copy instructions
 
 // row r of a (batch, key head) is query r / G, head r % G of the key head's G
 HV_DEV void hv_cross_row(const HvCrossArgs& a, int r, int kvh, int& query, int& column) {
@@ -115,23 +119,22 @@ HV_DEV void hv_wave_fence() {
 HV_DEV bf16x8 hv_bf16_ones() { return bf16x8{0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80}; }
 
 // ---- few states (Lk <= 16 NT <= 96, D <= 80): a prompt.  The stream of queries is what counts -- q is read once, o written once.
-// All of K and V^T of a (batch, key head) stay in a wave's REGISTERS as matrix operands.  A wave then streams tiles of ROWS queries
-// through two LDS slots of its own: the next tile is in flight by LDS-DMA while this one is computed, the results replace the
-// queries in the slot and leave it row by row.  (Straight from memory into operand registers the 16 lanes of an access lie in 16
-// rows -- 16 cache lines for 256 bytes: 133 us instead of XX at 2 x 147456 queries, 77 states, D = 40.)  A wave meets no barrier after the
-// states are loaded.  No running maximum: a row's scores are all there.  The number of 16-key tiles is a template argument:
-// branches around absent tiles cost more than a masked tile (twice the instructions).  G divides 32, so a lane's offsets inside a
-// tile are the same for every tile.
+// A workgroup takes four neighbouring query heads (4 / G key heads) and streams tiles of TQ queries through two LDS slots: the next
+// tile is in flight by LDS-DMA while this one is computed, the results replace the queries in the slot and leave it.  Both ways a
+// row's four heads are one run of memory (320 - 640 bytes).  At 2 x 147456 queries, 77 states, D = 40 (378 MB) the copies
+// alone take 85 us, all of it 103; a head at a time 99 / 115; straight from memory into operand registers (16 lanes in 16 rows) - / 133.
+// All of K and V^T of its key head stay in a wave's REGISTERS as matrix operands.  No running maximum: a row's scores are all there.
+// The number of 16-key tiles is a template argument: branches around absent tiles cost more than a masked tile.
 template <int D, int NT>
 __global__ __launch_bounds__(256, D == 40 ? 3 : 2) void hv_cross_attention_few_kernel(HvCrossArgs a) {
     using G = HvCrossGeom<D>;
     constexpr int KS = G::KS, DT = G::DT, P8 = G::P8, NP = (NT + 1) / 2, CH = 32 * NP;
-    constexpr int ROWS = HV_CROSS_FEW_ROWS(D), NI = ROWS * P8 / 64, SLOT = ROWS * D * 2;
-    static_assert(ROWS * P8 % 64 == 0, "whole copy instructions");
-    constexpr int STATES = CH * (G::KSTR + G::VSTR), SMEM = STATES > 8 * SLOT ? STATES : 8 * SLOT;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[SMEM];  // first the states, then 4 waves x 2 slots
+    constexpr int TQ = HV_CROSS_FEW_ROWS(D), NPC = 4 * P8, NI = TQ * NPC / 256, SLOT = TQ * NPC * 16;
+    static_assert(TQ * NPC % 256 == 0, "whole copy instructions per wave");
+    constexpr int VPART = 32 * G::VSTR;  // a wave's 32 rows of V, before the slots are used
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SLOT > 4 * VPART ? 2 * SLOT : 4 * VPART];
     __shared__ __attribute__((aligned(16))) float sBias[CH];
-    const int per_xcd = (a.units + 7) / 8;  // neighbouring units (the heads of one range of rows) on one XCD: they share cache lines
+    const int per_xcd = (a.units + 7) / 8;  // neighbouring units (the head groups of one range of rows) on one XCD
     const int unit = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per_xcd || unit >= a.units) return;
     const hv_cross_attention_params& p = a.p;
@@ -141,97 +144,110 @@ __global__ __launch_bounds__(256, D == 40 ? 3 : 2) void hv_cross_attention_few_k
 #else
     const int wave = tid >> 6;
 #endif
-    const int kvh = unit % p.kv_heads, group = unit / p.kv_heads % a.groups, b = unit / p.kv_heads / a.groups;
+    const int hgroups = p.heads / 4, hgroup = unit % hgroups, group = unit / hgroups % a.groups, b = unit / hgroups / a.groups;
+    const int kvh = (hgroup * 4 + wave) / a.G;
     int len = p.kv_len ? p.kv_len[b] : p.Lk;
     len = len < 0 ? 0 : len > p.Lk ? p.Lk : len;
     const u32x4 zero4 = {0u, 0u, 0u, 0u};
-    unsigned char* const sK = smem;
-    unsigned char* const sV = smem + CH * G::KSTR;
+    bf16x8 kf[NT][KS], vf[NP][DT];
     {
         const bf16_t* Kb = p.K + (long)b * p.k_stride_b + (long)kvh * D;
         const bf16_t* Vb = p.V + (long)b * p.v_stride_b + (long)kvh * D;
         const uint8_t* mask = p.key_mask ? p.key_mask + (long)b * p.mask_stride_b : nullptr;
-        constexpr int KP = KS * 4, VP = DT * 2;  // pieces of a padded row
-        for (int i = tid; i < CH * KP; i += 256) {
-            const int row = i / KP, piece = i % KP;
-            const bool on = row < len && piece < P8 && (mask == nullptr || mask[row] != 0);
-            hv_st16(sK + row * G::KSTR + piece * 16, on ? hv_ld16(Kb + (long)row * p.ldk + piece * 8) : zero4);
+        unsigned char* const part = smem + wave * VPART;
+        constexpr int VP = DT * 2;  // pieces of a padded V row
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt) {
+            const int row = kt * 16 + col;
+            const bool on = row < len && (mask == nullptr || mask[row] != 0);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                kf[kt][ks] = hv_as_bf16x8(on && ks * 32 + g * 8 < D ? hv_ld16(Kb + (long)row * p.ldk + ks * 32 + g * 8) : zero4);
         }
-        for (int i = tid; i < CH * VP; i += 256) {
-            const int row = i / VP, piece = i % VP;
-            const bool on = row < len && piece < P8 && (mask == nullptr || mask[row] != 0);
-            hv_st16(sV + row * G::VSTR + piece * 16, on ? hv_ld16(Vb + (long)row * p.ldv + piece * 8) : zero4);
+#pragma unroll
+        for (int pr = 0; pr < NP; ++pr) {
+            for (int i = lane; i < 32 * VP; i += 64) {
+                const int row = pr * 32 + i / VP, piece = i % VP;
+                const bool on = row < len && piece < P8 && (mask == nullptr || mask[row] != 0);
+                hv_st16(part + i / VP * G::VSTR + piece * 16, on ? hv_ld16(Vb + (long)row * p.ldv + piece * 8) : zero4);
+            }
+            hv_wave_fence();
+#pragma unroll
+            for (int d = 0; d < DT; ++d) vf[pr][d] = hv_cross_vfrag<D>(part, 0, d, col, g);
+            hv_wave_fence();
         }
         if (tid < CH) sBias[tid] = tid < len && (mask == nullptr || mask[tid] != 0) ? 0.f : -INFINITY;
     }
-    __syncthreads();
-    bf16x8 kf[NT][KS], vf[NP][DT];
-#pragma unroll
-    for (int kt = 0; kt < NT; ++kt)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) kf[kt][ks] = hv_as_bf16x8(hv_ld16(sK + (kt * 16 + col) * G::KSTR + ks * 64 + g * 16));
-#pragma unroll
-    for (int pr = 0; pr < NP; ++pr)
-#pragma unroll
-        for (int d = 0; d < DT; ++d) vf[pr][d] = hv_cross_vfrag<D>(sV, pr * 32, d, col, g);
-    __syncthreads();  // every wave has its operands: the slots may be written
+    hv_barrier_raw();  // every wave has its operands (the barrier waits for LDS reads): copies may land in the slots
 
-    // slot layout: row major, 16-byte pieces; rows of 128 bytes (D = 64) with their pieces XOR-swizzled, as their fragment reads would
-    // all start in the same banks (rows of 80 and 160 bytes do not)
-    auto slot_of = [](int row, int piece) { return (row * P8 + (D == 64 ? piece ^ (row & 7) : piece)) * 16; };
-    const int end = min((group + 1) * a.per_wg, a.blocks);  // tiles of ROWS rows
-    const bf16_t* const Qb = p.Q + (long)b * p.q_stride_b + (long)kvh * a.G * D;
-    bf16_t* const Ob = p.O + (long)b * p.o_stride_b + (long)kvh * a.G * D;
+    // slot layout: query-major, NPC 16-byte pieces a query (its four heads), rotated by a function of the query so that the 16 rows of a
+    // fragment access lie in 16 different quarters of the banks: NPC = 20, 32, 40 repeat after 4, 1, 2 queries
+    constexpr int SH = NPC % 32 == 0 ? 0 : NPC % 8 == 0 ? 1 : 2;
+    auto rotated = [](int query, int piece) {
+        const int at = piece + ((query >> SH) & (15 >> SH));
+        return at < NPC ? at : at - NPC;
+    };
+    const bf16_t* const Qb = p.Q + (long)b * p.q_stride_b + (long)hgroup * 4 * D;
+    bf16_t* const Ob = p.O + (long)b * p.o_stride_b + (long)hgroup * 4 * D;
     auto offset = [&](int i, int last, long ld) {  // byte offset inside a tile of the piece that lane and instruction i carry
-        const int idx = i * 64 + lane, slot = idx % P8;
-        int row = idx / P8;
-        const int piece = D == 64 ? slot ^ (row & 7) : slot;
-        row = min(row, last);
-        const int query = a.G == 1 ? row : row / a.G;
-        return (unsigned)query * (unsigned)(ld * 2) + (unsigned)((row - query * a.G) * D * 2 + piece * 16);
+        const int idx = (wave * NI + i) * 64 + lane, slot = idx % NPC, query = idx / NPC;
+        int piece = slot - ((query >> SH) & (15 >> SH));
+        piece = piece < 0 ? piece + NPC : piece;
+        return (unsigned)min(query, last) * (unsigned)(ld * 2) + (unsigned)(piece * 16);
     };
     unsigned qofs[NI], oofs[NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-        qofs[i] = offset(i, ROWS, p.ldq);
-        oofs[i] = offset(i, ROWS, p.ldo);
+        qofs[i] = offset(i, TQ, p.ldq);
+        oofs[i] = offset(i, TQ, p.ldo);
     }
-    auto issue = [&](int tile, unsigned char* slot) {
-        const char* base = (const char*)(Qb + (long)(tile * ROWS / a.G) * p.ldq);
-        const int last = a.rows - 1 - tile * ROWS;
-        if (last >= ROWS - 1) {
+    unsigned char* slot = smem;
+    unsigned char* other = smem + SLOT;
+    auto issue = [&](int tile, unsigned char* to) {
+        const char* base = (const char*)(Qb + (long)tile * TQ * p.ldq);
+        const int last = p.Lq - 1 - tile * TQ;
+        if (last >= TQ - 1) {
 #pragma unroll
-            for (int i = 0; i < NI; ++i) hv_glds16_s(base, qofs[i], slot + i * 1024);
-        } else {  // rows behind the last repeat it and are not stored
+            for (int i = 0; i < NI; ++i) hv_glds16_s(base, qofs[i], to + (wave * NI + i) * 1024);
+        } else {  // queries behind the last repeat it and are not stored
 #pragma unroll
-            for (int i = 0; i < NI; ++i) hv_glds16_s(base, offset(i, last, p.ldq), slot + i * 1024);
+            for (int i = 0; i < NI; ++i) hv_glds16_s(base, offset(i, last, p.ldq), to + (wave * NI + i) * 1024);
         }
     };
-    unsigned char* slot = smem + wave * 2 * SLOT;
-    unsigned char* other = slot + SLOT;
-    int tile = group * a.per_wg + wave;
-    if (tile < end) issue(tile, slot);
-    for (bool first = true; tile < end; tile += 4, first = false) {
+    // rows of this wave: the G query heads of its key head are G waves' rows, TQ each; row r = wave's share * TQ + i of them is query
+    // r / G, head r % G
+    const int share = wave % a.G;
+    const int end = min((group + 1) * a.per_wg, a.blocks);  // tiles of TQ queries
+    int tile = group * a.per_wg;
+    issue(tile, slot);
+    for (bool first = true; tile < end; ++tile, first = false) {
         // in flight, in order: this tile's copies, the stores of the tile before (all NI of them: it was not the last)
         if (first) hv_vm_wait<0>();
         else hv_vm_wait<NI>();
-        hv_wave_fence();
-        if (tile + 4 < end) issue(tile + 4, other);
+        hv_barrier_raw();  // the tile is there, and nobody reads the other slot any more
+        if (tile + 1 < end) issue(tile + 1, other);
 #pragma unroll 1
-        for (int sub = 0; sub < ROWS; sub += 16) {
+        for (int sub = 0; sub < TQ; sub += 16) {
+            int query = sub + col, head = wave;
+            if (a.G > 1) {  // (uniform)
+                const int r = share * TQ + query;
+                query = r / a.G;
+                head = wave - share + r % a.G;
+            }
+            unsigned char* const row = slot + query * (NPC * 16);
             f32x4 s[NT];
 #pragma unroll
             for (int kt = 0; kt < NT; ++kt) s[kt] = *reinterpret_cast<const f32x4*>(sBias + kt * 16 + g * 4);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 u32x4 q = zero4;
-                if ((ks + 1) * 32 <= D || ks * 32 + g * 8 < D) q = hv_ld16(slot + slot_of(sub + col, ks * 4 + g));
+                if ((ks + 1) * 32 <= D || ks * 32 + g * 8 < D) q = hv_ld16(row + rotated(query, head * P8 + ks * 4 + g) * 16);
 #pragma unroll
                 for (int kt = 0; kt < NT; ++kt) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kt][ks], hv_as_bf16x8(q), s[kt], 0, 0, 0);
             }
             float top = -INFINITY;
 #pragma unroll
-            for (int kt = 0; kt < NT; ++kt) top = fmaxf(fmaxf(top, fmaxf(s[kt][0], s[kt][1])), fmaxf(s[kt][2], s[kt][3]));
+            for (int kt = 0; kt < NT; ++kt) top = hv_max5(top, s[kt]);
             top = hv_max_quarters(top);
             const float mc = top == -INFINITY ? 0.f : -top * a.c;  // nothing attended: 2^(-inf - 0) = 0
             f32x4 acc[DT], sum;
@@ -253,18 +269,18 @@ __global__ __launch_bounds__(256, D == 40 ? 3 : 2) void hv_cross_attention_few_k
 #pragma unroll
                 for (int d = 0; d < DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[pr][d], pf, pr ? acc[d] : none, 0, 0, 0);
             }
+            // (the pieces of these rows and heads are this wave's alone, and it has read them)
             hv_wave_fence();
-            hv_cross_store<D>([&](int piece) { return slot + slot_of(sub + col, piece); }, acc, sum[0], g);
+            hv_cross_store<D>([&](int piece) { return row + rotated(query, head * P8 + piece) * 16; }, acc, sum[0], g);
         }
-        hv_wave_fence();
-        char* base = (char*)(Ob + (long)(tile * ROWS / a.G) * p.ldo);
+        hv_barrier_raw();  // the results of all four waves are in the slot
+        char* base = (char*)(Ob + (long)tile * TQ * p.ldo);
         u32x4 out[NI];
 #pragma unroll
-        for (int i = 0; i < NI; ++i) out[i] = hv_ld16(slot + i * 1024 + lane * 16);
+        for (int i = 0; i < NI; ++i) out[i] = hv_ld16(slot + (wave * NI + i) * 1024 + lane * 16);
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-            if (tile * ROWS + (i * 64 + lane) / P8 < a.rows) hv_st16(base + oofs[i], out[i]);
-        hv_wave_fence();  // (the stores wait for their data: the slot is free when they are issued)
+            if (tile * TQ + ((wave * NI + i) * 64 + lane) / NPC < p.Lq) hv_st16(base + oofs[i], out[i]);
         unsigned char* const t = slot;
         slot = other;
         other = t;
@@ -387,14 +403,13 @@ __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_atte
                         for (int t = 0; t < QT; ++t) s[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][ks], s[t][kt], 0, 0, 0);
                     }
 #pragma unroll
-                    for (int t = 0; t < QT; ++t)
-                        top[t] = fmaxf(fmaxf(top[t], fmaxf(s[t][kt][0], s[t][kt][1])), fmaxf(s[t][kt][2], s[t][kt][3]));
+                    for (int t = 0; t < QT; ++t) top[t] = hv_max5(top[t], s[t][kt]);
                 }
             }
             float mc[QT];
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                const float mn = fmaxf(m[t], hv_max_quarters(top[t]));
+                const float mn = hv_max(m[t], hv_max_quarters(top[t]));
                 const float ms = mn == -INFINITY ? 0.f : mn;  // nothing attended yet: 2^(-inf - 0) = 0, not 2^(-inf + inf)
                 const float alpha = __builtin_amdgcn_exp2f((m[t] - ms) * a.c);
                 m[t] = mn;
@@ -467,7 +482,7 @@ __global__ __launch_bounds__(256) void hv_cross_attention_join_kernel(HvCrossArg
     const int kvh = (int)(item / a.rows % p.kv_heads), b = (int)(item / a.rows / p.kv_heads);
     const float* src = p.workspace + item * a.splits * (D + 2);
     float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, src[s * (D + 2)]);
+    for (int s = 0; s < a.splits; ++s) m = hv_max(m, src[s * (D + 2)]);
     const float ms = m == -INFINITY ? 0.f : m;
     float l = 0.f, o[(D + 63) / 64];
 #pragma unroll
@@ -501,14 +516,16 @@ static inline int hv_cross_attention_plan(const hv_cross_attention_params& p, Hv
     a.splits = 1;
     a.c = p.scale * 1.44269504088896341f;
     long units;
-    a.few = p.Lk <= 96 && p.D <= 80 && 32 % a.G == 0 && p.ldq < (1L << 24) && p.ldo < (1L << 24);
-    if (a.few) {  // ranges of tiles for about four rounds of the workgroups that fit the chip
+    a.few = p.Lk <= 96 && p.D <= 80 && p.heads % 4 == 0 && 4 % a.G == 0 && p.ldq < (1L << 24) && p.ldo < (1L << 24);
+    if (a.few) {  // as many ranges of tiles as workgroups fit the chip at once: each pays for its states once
         const int tile = HV_CROSS_FEW_ROWS(p.D);
-        a.blocks = (int)((rows + tile - 1) / tile);
-        const long fit = 256L * (p.D == 40 ? 3 : 2), groups = (fit * 4 + pairs - 1) / (pairs > 0 ? pairs : 1);
+        a.blocks = (p.Lq + tile - 1) / tile;
+        const long lists = (long)p.B * (p.heads / 4), fit = 256L * (p.D == 40 ? 3 : 2);
+        const long groups = lists > 0 && fit > lists ? fit / lists : 1;
         a.per_wg = (int)((a.blocks + groups - 1) / groups);
-        a.per_wg = (a.per_wg + 3) / 4 * 4;
-        if (a.per_wg < 4) a.per_wg = 4;
+        if (a.per_wg < 1) a.per_wg = 1;
+        a.groups = (a.blocks + a.per_wg - 1) / a.per_wg;
+        units = lists * a.groups;
     } else {
         a.qt = rows > 64 ? 2 : 1;
         a.blocks = (int)((rows + 64 * a.qt - 1) / (64 * a.qt));
@@ -519,9 +536,9 @@ static inline int hv_cross_attention_plan(const hv_cross_attention_params& p, Hv
             a.splits = (int)(want < most ? want : most);
             if (a.splits < 1) a.splits = 1;
         }
+        a.groups = a.blocks;
+        units = pairs * a.groups * a.splits;
     }
-    a.groups = (a.blocks + a.per_wg - 1) / a.per_wg;
-    units = pairs * a.groups * a.splits;
     if (units > 0x3fffffffL) return -1;
     a.units = (int)units;
     return 0;

@@ -33,6 +33,13 @@ def cx():
     (2, 9, 257, 2, 2, 160, "len", "plain"),      # keys cut into ranges
     (2, 1, 530, 4, 1, 128, "both", "fused"),     # shared key head, one query
     (3, 2, 0, 2, 2, 40, None, "plain"),          # no states at all
+    (2, 1, 3, 4, 4, 40, "len", "plain"),         # four heads a workgroup, states in registers
+    (1, 131, 77, 4, 4, 40, "mask", "wide"),      # several tiles, the last one ragged
+    (2, 70, 33, 4, 2, 64, "both", "fused"),      # shared key heads: two waves of rows each
+    (1, 35, 96, 4, 1, 80, "len", "inplace"),     # one key head for all four
+    (1, 33, 80, 8, 8, 64, None, "shared"),
+    (2, 40, 17, 4, 4, 80, "mask", "plain"),
+    (3, 5, 0, 4, 4, 40, None, "plain"),
 ])
 def test_cross_attention(cx, B, Lq, Lk, heads, kv_heads, D, mask, layout):
     oc.case_cross(cx, B, Lq, Lk, heads, kv_heads, D, mask, seed=Lk + D, layout=layout)
