@@ -46,13 +46,14 @@ HV_DEV float hv_max_quarters(float x) {
 
 struct HvCrossArgs {
     hv_cross_attention_params p;
-    int G, rows;         // heads per key head; Lq * G
-    int blocks, per_wg;  // row blocks of a (batch, key head); consecutive blocks one workgroup takes
-    int groups;          // ceil(blocks / per_wg)
-    int units;           // workgroups with work
-    int splits;          // ranges the keys are cut into
-    int few, qt;         // which kernel; its 16-row tiles per wave
     float c;             // scale * log2 e
+    int G, rows;         // heads per key head; rows of a (batch, key head): Lq * G
+    int kernel;          // 0: few states, 1: few rows, 2: any, one 16-row tile per wave, 3: any, two
+    int blocks;          // row blocks of a (batch, key head); few states: tiles of queries
+    int per_wg, groups;  // few states: tiles one workgroup takes, workgroups per entry and head group
+    int splits, per;     // ranges the keys are cut into, keys per range
+    int run;             // neighbouring units that go to one XCD
+    int units;           // workgroups with work
 };
 
 #define HV_CROSS_FEW_ROWS(D) ((D) == 40 ? 64 : 32)  // hv_cross_attention_few_kernel: queries whose pieces fill whole copy instructions
@@ -105,6 +106,16 @@ HV_DEV void hv_cross_store(At at, const f32x4* acc, float sum, int g) {
             hv_st8((char*)at(d * 2 + g / 2) + (g & 1) * 8, u32x2{hv_pack2(acc[d][0] * inv, acc[d][1] * inv), hv_pack2(acc[d][2] * inv, acc[d][3] * inv)});
     }
 }
+
+#ifndef HV_EMU
+HV_DEV unsigned long hv_ballot(bool x) { return __ballot(x); }
+#else
+HV_DEV unsigned long hv_ballot(bool x) {
+    unsigned long r = 0;
+    for (int i = 0; i < 64; ++i) r |= (unsigned long)(__shfl((int)x, i) != 0) << i;
+    return r;
+}
+#endif
 
 // between a wave's own LDS writes and other lanes' reads of them: the LDS serves a wave in order, the compiler has to keep that order
 HV_DEV void hv_wave_fence() {
@@ -287,36 +298,54 @@ __global__ __launch_bounds__(256, D == 40 ? 3 : 2) void hv_cross_attention_few_k
     }
 }
 
-template <int D, int QT, int NP>
+// which part of the work a workgroup of the kernels below takes.  The states of a (batch, key head) are read by all of its row
+// blocks and should stay in one L2: neighbouring units (row blocks of the same keys, in runs of a.run) go to one XCD, the runs to the
+// XCDs in turn, so that entries of different lengths spread over all of them.  The keys are cut into ranges of a.per keys
+// whatever an entry's length: workgroups are equally long, those behind an entry's end leave at once.
+struct HvCrossPart {
+    int b, kvh, block, split, begin, end;
+    bool none;
+};
+HV_DEV HvCrossPart hv_cross_part(const HvCrossArgs& a) {
+    const hv_cross_attention_params& p = a.p;
+    const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+    const int run = (at / a.run) * 8 + xcd, unit = run * a.run + at % a.run;
+    HvCrossPart w;
+    w.none = unit >= a.units;
+    w.block = unit % a.blocks;
+    int rest = unit / a.blocks;
+    w.split = rest % a.splits;
+    rest /= a.splits;
+    w.kvh = rest % p.kv_heads;
+    w.b = w.none ? 0 : rest / p.kv_heads;
+    int len = p.kv_len ? p.kv_len[w.b] : p.Lk;
+    len = len < 0 ? 0 : len > p.Lk ? p.Lk : len;
+    w.begin = min(w.split * a.per, len);
+    w.end = min(w.begin + a.per, len);
+    w.none = w.none || (w.split > 0 && w.begin >= w.end);  // (the join does not read it; range 0 is always there)
+    return w;
+}
+
+// The running maximum is moved only where a score passes it by more than 2^8: the weights then stay below 2^8, their sums far inside
+// fp32, and the products by 2^((m - m') c) are rare after the first chunk.
+#define HV_CROSS_SLACK 8.0f
+
+// ---- any number of states: a workgroup's 64 QT rows go through the keys in chunks of 64, staged in LDS for all four waves, the next
+// chunk on its way in registers.
+template <int D, int QT>
 __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_attention_kernel(HvCrossArgs a) {
     using Geom = HvCrossGeom<D>;
-    constexpr int KS = Geom::KS, DT = Geom::DT, P8 = Geom::P8, CH = 32 * NP, KSTR = Geom::KSTR, VSTR = Geom::VSTR;
-    constexpr int NV = (CH * P8 + 255) / 256;              // 16-byte pieces of K (and of V) that a thread stages
+    constexpr int KS = Geom::KS, DT = Geom::DT, P8 = Geom::P8, CH = 64, KSTR = Geom::KSTR, VSTR = Geom::VSTR;
+    constexpr int NV = (CH * P8 + 255) / 256;  // 16-byte pieces of K (and of V) that a thread stages
     __shared__ __attribute__((aligned(16))) unsigned char sK[CH * KSTR];
     __shared__ __attribute__((aligned(16))) unsigned char sV[CH * VSTR];
     __shared__ __attribute__((aligned(16))) float sBias[CH];
-
-    // neighbouring units (the heads of one row block, then the next row blocks) run on one XCD: their query rows share cache lines
-    const int per_xcd = (a.units + 7) / 8;
-    const int unit = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per_xcd || unit >= a.units) return;
+    const HvCrossPart part = hv_cross_part(a);
+    if (part.none) return;
     const hv_cross_attention_params& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
-    const int kvh = unit % p.kv_heads;
-    int rest = unit / p.kv_heads;
-    const int split = rest % a.splits;
-    rest /= a.splits;
-    const int group = rest % a.groups, b = rest / a.groups;
-
-    int len = p.kv_len ? p.kv_len[b] : p.Lk;
-    len = len < 0 ? 0 : len > p.Lk ? p.Lk : len;
-    int k_begin = 0, k_end = len;
-    if (a.splits > 1) {
-        const int per = ((len + a.splits - 1) / a.splits + 31) / 32 * 32;
-        k_begin = min(split * per, len);
-        k_end = min(k_begin + per, len);
-    }
-    const int chunks = (k_end - k_begin + CH - 1) / CH;
+    const int b = part.b, kvh = part.kvh, k_end = part.end;
+    const int chunks = (k_end - part.begin + CH - 1) / CH;
     const bf16_t* Kb = p.K + (long)b * p.k_stride_b + (long)kvh * D;
     const bf16_t* Vb = p.V + (long)b * p.v_stride_b + (long)kvh * D;
     const uint8_t* mask = p.key_mask ? p.key_mask + (long)b * p.mask_stride_b : nullptr;
@@ -357,59 +386,62 @@ __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_atte
         }
         if (tid < CH) sBias[tid] = breg;
     };
-    fetch(k_begin);
-    {
-        const int r0 = (group * 4 + wave) * QT * 16 + col;
-        bf16x8 qf[QT][KS];
+    fetch(part.begin);
+
+    const int r0 = (part.block * 4 + wave) * QT * 16 + col;
+    bf16x8 qf[QT][KS];
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            const int r = r0 + t * 16;
-            int query, column;
-            hv_cross_row(a, r, kvh, query, column);
-            const bf16_t* src = p.Q + (long)b * p.q_stride_b + (long)query * p.ldq + column;
+    for (int t = 0; t < QT; ++t) {
+        const int r = r0 + t * 16;
+        int query, column;
+        hv_cross_row(a, r, kvh, query, column);
+        const bf16_t* src = p.Q + (long)b * p.q_stride_b + (long)query * p.ldq + column;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-                qf[t][ks] = hv_as_bf16x8(r < a.rows && ks * 32 + g * 8 < D ? hv_ld16(src + ks * 32 + g * 8) : zero4);
-        }
-        f32x4 acc[QT][DT], lsum[QT];
-        float m[QT];
+        for (int ks = 0; ks < KS; ++ks)
+            qf[t][ks] = hv_as_bf16x8(r < a.rows && ks * 32 + g * 8 < D ? hv_ld16(src + ks * 32 + g * 8) : zero4);
+    }
+    f32x4 acc[QT][DT], lsum[QT];
+    float m[QT], mc[QT];
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            m[t] = -INFINITY;
-            lsum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < QT; ++t) {
+        m[t] = -INFINITY;
+        mc[t] = 0.f;
+        lsum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        for (int ch = 0; ch < chunks; ++ch) {
-            const int n = k_end - k_begin - ch * CH;  // keys left
-            if (ch > 0) __syncthreads();  // the readers of the previous chunk are done
-            stage();
-            __syncthreads();
-            if (ch + 1 < chunks) fetch(k_begin + (ch + 1) * CH);
-            f32x4 s[QT][2 * NP];
-            float top[QT];
+        for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int ch = 0; ch < chunks; ++ch) {
+        if (ch > 0) __syncthreads();  // the readers of the previous chunk are done
+        stage();
+        __syncthreads();
+        if (ch + 1 < chunks) fetch(part.begin + (ch + 1) * CH);
+        f32x4 s[QT][4];
 #pragma unroll
-            for (int t = 0; t < QT; ++t) top[t] = -INFINITY;
+        for (int kt = 0; kt < 4; ++kt) {
+            const f32x4 bias = *reinterpret_cast<const f32x4*>(sBias + kt * 16 + g * 4);
 #pragma unroll
-            for (int kt = 0; kt < 2 * NP; ++kt) {
-                if ((kt & ~1) * 16 < n) {
-                    const f32x4 bias = *reinterpret_cast<const f32x4*>(sBias + kt * 16 + g * 4);
+            for (int t = 0; t < QT; ++t) s[t][kt] = bias;
 #pragma unroll
-                    for (int t = 0; t < QT; ++t) s[t][kt] = bias;
+            for (int ks = 0; ks < KS; ++ks) {
+                const bf16x8 kf = hv_as_bf16x8(hv_ld16(sK + (kt * 16 + col) * KSTR + ks * 64 + g * 16));
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        const bf16x8 kf = hv_as_bf16x8(hv_ld16(sK + (kt * 16 + col) * KSTR + ks * 64 + g * 16));
-#pragma unroll
-                        for (int t = 0; t < QT; ++t) s[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][ks], s[t][kt], 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int t = 0; t < QT; ++t) top[t] = hv_max5(top[t], s[t][kt]);
-                }
+                for (int t = 0; t < QT; ++t) s[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][ks], s[t][kt], 0, 0, 0);
             }
-            float mc[QT];
+        }
+        float top[QT];
+        bool past = false;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            top[t] = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) top[t] = hv_max5(top[t], s[t][kt]);
+            top[t] = hv_max_quarters(top[t]);
+            past = past || (top[t] - m[t]) * a.c > HV_CROSS_SLACK;
+        }
+        if (__any(past)) {
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                const float mn = hv_max(m[t], hv_max_quarters(top[t]));
+                const float mn = hv_max(m[t], top[t]);
                 const float ms = mn == -INFINITY ? 0.f : mn;  // nothing attended yet: 2^(-inf - 0) = 0, not 2^(-inf + inf)
                 const float alpha = __builtin_amdgcn_exp2f((m[t] - ms) * a.c);
                 m[t] = mn;
@@ -421,57 +453,201 @@ __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_atte
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[t][d][e] *= alpha;
             }
-#pragma unroll
-            for (int pr = 0; pr < NP; ++pr) {
-                if (pr * 32 < n) {
-                    bf16x8 pf[QT];
-#pragma unroll
-                    for (int t = 0; t < QT; ++t) {
-                        float f[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = __builtin_amdgcn_exp2f(fmaf(s[t][2 * pr + e / 4][e % 4], a.c, mc[t]));
-                        pf[t] = hv_as_bf16x8(hv_pack8(f));
-                    }
-#pragma unroll
-                    for (int t = 0; t < QT; ++t) lsum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_bf16_ones(), pf[t], lsum[t], 0, 0, 0);
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        const bf16x8 vf = hv_cross_vfrag<D>(sV, pr * 32, d, col, g);
-#pragma unroll
-                        for (int t = 0; t < QT; ++t) acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], acc[t][d], 0, 0, 0);
-                    }
-                }
-            }
         }
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            const int r = r0 + t * 16;
-            if (r >= a.rows) continue;
-            if (a.splits > 1) {  // unnormalised sums, with the maximum and the sum of weights they refer to
-                float* dst = p.workspace + ((((long)b * p.kv_heads + kvh) * a.rows + r) * a.splits + split) * (D + 2);
+        for (int pr = 0; pr < 2; ++pr) {
+            bf16x8 pf[QT];
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const int at = d < Geom::PAIRED ? d / 2 * 32 + g * 8 + (d & 1) * 4 : d * 16 + g * 4;
-                    if (at < D) {
+            for (int t = 0; t < QT; ++t) {
+                float f[8];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) dst[2 + at + e] = acc[t][d][e];
-                    }
-                }
-                if (g == 0) {
-                    dst[0] = m[t];
-                    dst[1] = lsum[t][0];
-                }
-            } else {
-                int query, column;
-                hv_cross_row(a, r, kvh, query, column);
-                bf16_t* dst = p.O + (long)b * p.o_stride_b + (long)query * p.ldo + column;
-                hv_cross_store<D>([&](int piece) { return dst + piece * 8; }, acc[t], lsum[t][0], g);
+                for (int e = 0; e < 8; ++e) f[e] = __builtin_amdgcn_exp2f(fmaf(s[t][2 * pr + e / 4][e % 4], a.c, mc[t]));
+                pf[t] = hv_as_bf16x8(hv_pack8(f));
             }
+#pragma unroll
+            for (int t = 0; t < QT; ++t) lsum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_bf16_ones(), pf[t], lsum[t], 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const bf16x8 vf = hv_cross_vfrag<D>(sV, pr * 32, d, col, g);
+#pragma unroll
+                for (int t = 0; t < QT; ++t) acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], acc[t][d], 0, 0, 0);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int r = r0 + t * 16;
+        if (r >= a.rows) continue;
+        if (a.splits > 1) {  // unnormalised sums, with the maximum and the sum of weights they refer to
+            float* dst = p.workspace + ((((long)b * p.kv_heads + kvh) * a.rows + r) * a.splits + part.split) * (D + 2);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const int at = d < Geom::PAIRED ? d / 2 * 32 + g * 8 + (d & 1) * 4 : d * 16 + g * 4;
+                if (at < D) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dst[2 + at + e] = acc[t][d][e];
+                }
+            }
+            if (g == 0) {
+                dst[0] = m[t];
+                dst[1] = lsum[t][0];
+            }
+        } else {
+            int query, column;
+            hv_cross_row(a, r, kvh, query, column);
+            bf16_t* dst = p.O + (long)b * p.o_stride_b + (long)query * p.ldo + column;
+            hv_cross_store<D>([&](int piece) { return dst + piece * 8; }, acc[t], lsum[t][0], g);
         }
     }
 }
 
-// joins the splits of a row: o = sum_s o_s 2^((m_s - m) c) / sum_s l_s 2^((m_s - m) c); one wavefront per row
+// ---- at most 16 rows (Lq G <= 16): reading the states is all there is.  The four waves of a workgroup take blocks of 32 keys in turn,
+// each on its own: K straight from memory into operand registers, V through 32 rows of LDS of its own (for the transposed read), both
+// requested a block ahead -- 16 KB in flight per wave at D = 128, and no barrier until the four results are joined in LDS.
+template <int D>
+__global__ __launch_bounds__(256, 2) void hv_cross_attention_rows_kernel(HvCrossArgs a) {
+    using Geom = HvCrossGeom<D>;
+    constexpr int KS = Geom::KS, DT = Geom::DT, P8 = Geom::P8, VSTR = Geom::VSTR;
+    constexpr int NV = (32 * P8 + 63) / 64;  // 16-byte pieces of V per lane and block
+    constexpr int VPART = 32 * VSTR, JOIN = 16 * (D + 2) * 4;
+    constexpr int OWN = VPART > JOIN ? VPART : JOIN;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[4 * OWN];
+    const HvCrossPart part = hv_cross_part(a);
+    if (part.none) return;
+    const hv_cross_attention_params& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+    const int b = part.b, kvh = part.kvh;
+    const bf16_t* Kb = p.K + (long)b * p.k_stride_b + (long)kvh * D;
+    const bf16_t* Vb = p.V + (long)b * p.v_stride_b + (long)kvh * D;
+    const uint8_t* mask = p.key_mask ? p.key_mask + (long)b * p.mask_stride_b : nullptr;
+    unsigned char* const sV = smem + wave * OWN;
+    const u32x4 zero4 = {0u, 0u, 0u, 0u};
+    if constexpr (DT * 2 > P8) {
+        if (lane < 32) hv_st16(sV + lane * VSTR + P8 * 16, zero4);
+    }
+    bf16x8 qf[KS];
+    {
+        int query, column;
+        hv_cross_row(a, col, kvh, query, column);
+        const bf16_t* src = p.Q + (long)b * p.q_stride_b + (long)query * p.ldq + column;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            qf[ks] = hv_as_bf16x8(col < a.rows && ks * 32 + g * 8 < D ? hv_ld16(src + ks * 32 + g * 8) : zero4);
+    }
+    f32x4 acc[DT], lsum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, mc = 0.f;
+    u32x4 kreg[2][KS], vreg[NV];
+    bool on[2] = {false, false};  // whether this lane's key of a 16-key tile (its col) is attended
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int row = k0 + t * 16 + col;
+            on[t] = row < part.end && (mask == nullptr || mask[row] != 0);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                kreg[t][ks] = row < part.end && ks * 32 + g * 8 < D ? hv_ld16(Kb + (long)row * p.ldk + ks * 32 + g * 8) : zero4;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = i * 64 + lane, row = k0 + idx / P8;
+            vreg[i] = idx < 32 * P8 && row < part.end ? hv_ld16(Vb + (long)row * p.ldv + idx % P8 * 8) : zero4;
+        }
+    };
+    int k0 = part.begin + wave * 32;
+    if (k0 < part.end) fetch(k0);
+    for (; k0 < part.end; k0 += 128) {
+        // bit j: key k0 + j is attended (lanes 0 - 15 hold the tile's keys)
+        unsigned keep = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) keep |= (unsigned)(hv_ballot(on[t]) & 0xffffu) << (16 * t);
+        f32x4 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] = keep >> (t * 16 + g * 4 + e) & 1u ? 0.f : -INFINITY;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_as_bf16x8(on[t] ? kreg[t][ks] : zero4), qf[ks], s[t], 0, 0, 0);
+        }
+        hv_wave_fence();
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = i * 64 + lane, row = idx / P8;
+            if (idx < 32 * P8) hv_st16(sV + row * VSTR + idx % P8 * 16, keep >> row & 1u ? vreg[i] : zero4);
+        }
+        hv_wave_fence();
+        if (k0 + 128 < part.end) fetch(k0 + 128);
+        float top = hv_max_quarters(hv_max5(hv_max5(-INFINITY, s[0]), s[1]));
+        if (__any((top - m) * a.c > HV_CROSS_SLACK)) {
+            const float mn = hv_max(m, top), ms = mn == -INFINITY ? 0.f : mn;
+            const float alpha = __builtin_amdgcn_exp2f((m - ms) * a.c);
+            m = mn;
+            mc = -ms * a.c;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) lsum[e] *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[d][e] *= alpha;
+        }
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = __builtin_amdgcn_exp2f(fmaf(s[e / 4][e % 4], a.c, mc));
+        const bf16x8 pf = hv_as_bf16x8(hv_pack8(f));
+        lsum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_bf16_ones(), pf, lsum, 0, 0, 0);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_cross_vfrag<D>(sV, 0, d, col, g), pf, acc[d], 0, 0, 0);
+    }
+    // the four waves' results: [wave][row][m, l, D sums]
+    __syncthreads();
+    float* const mine = reinterpret_cast<float*>(smem) + (wave * 16 + col) * (D + 2);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+        const int at = d < Geom::PAIRED ? d / 2 * 32 + g * 8 + (d & 1) * 4 : d * 16 + g * 4;
+        if (at < D) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mine[2 + at + e] = acc[d][e];
+        }
+    }
+    if (g == 0) {
+        mine[0] = m;
+        mine[1] = lsum[0];
+    }
+    __syncthreads();
+    for (int i = tid; i < a.rows * D; i += 256) {
+        const int r = i / D, d = i - r * D;
+        const float* src = reinterpret_cast<const float*>(smem) + r * (D + 2);
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = hv_max(top, src[w * 16 * (D + 2)]);
+        const float ms = top == -INFINITY ? 0.f : top;
+        float l = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float* q = src + w * 16 * (D + 2);
+            const float x = __builtin_amdgcn_exp2f((q[0] - ms) * a.c);
+            l += x * q[1];
+            o += x * q[2 + d];
+        }
+        if (a.splits > 1) {
+            float* dst = p.workspace + ((((long)b * p.kv_heads + kvh) * a.rows + r) * a.splits + part.split) * (D + 2);
+            dst[2 + d] = o;
+            if (d == 0) {
+                dst[0] = top;
+                dst[1] = l;
+            }
+        } else {
+            int query, column;
+            hv_cross_row(a, r, kvh, query, column);
+            (p.O + (long)b * p.o_stride_b + (long)query * p.ldo + column)[d] = hv_f2bf(l == 0.f ? 0.f : o / l);
+        }
+    }
+}
+
+// joins the ranges of a row: o = sum_s o_s 2^((m_s - m) c) / sum_s l_s 2^((m_s - m) c); one wavefront per row
 template <int D>
 __global__ __launch_bounds__(256) void hv_cross_attention_join_kernel(HvCrossArgs a) {
     const hv_cross_attention_params& p = a.p;
@@ -481,13 +657,16 @@ __global__ __launch_bounds__(256) void hv_cross_attention_join_kernel(HvCrossArg
     const int r = (int)(item % a.rows);
     const int kvh = (int)(item / a.rows % p.kv_heads), b = (int)(item / a.rows / p.kv_heads);
     const float* src = p.workspace + item * a.splits * (D + 2);
+    int len = p.kv_len ? p.kv_len[b] : p.Lk;
+    len = len > p.Lk ? p.Lk : len;
+    const int ranges = len <= a.per ? 1 : (len + a.per - 1) / a.per;  // those behind the entry's end wrote nothing
     float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = hv_max(m, src[s * (D + 2)]);
+    for (int s = 0; s < ranges; ++s) m = hv_max(m, src[s * (D + 2)]);
     const float ms = m == -INFINITY ? 0.f : m;
     float l = 0.f, o[(D + 63) / 64];
 #pragma unroll
     for (int i = 0; i < (D + 63) / 64; ++i) o[i] = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
+    for (int s = 0; s < ranges; ++s) {
         const float* q = src + s * (D + 2);
         const float w = __builtin_amdgcn_exp2f((q[0] - ms) * a.c);
         l += w * q[1];
@@ -513,11 +692,13 @@ static inline int hv_cross_attention_plan(const hv_cross_attention_params& p, Hv
     a.p = p;
     a.G = p.heads / p.kv_heads;
     a.rows = (int)rows;
-    a.splits = 1;
     a.c = p.scale * 1.44269504088896341f;
+    a.splits = a.run = a.per_wg = a.groups = 1;
+    a.per = p.Lk;
     long units;
-    a.few = p.Lk <= 96 && p.D <= 80 && p.heads % 4 == 0 && 4 % a.G == 0 && p.ldq < (1L << 24) && p.ldo < (1L << 24);
-    if (a.few) {  // as many ranges of tiles as workgroups fit the chip at once: each pays for its states once
+    if (p.Lk <= 96 && p.D <= 80 && p.heads % 4 == 0 && 4 % a.G == 0 && p.ldq < (1L << 24) && p.ldo < (1L << 24)) {
+        // as many ranges of tiles as workgroups fit the chip at once: each pays for its states once
+        a.kernel = 0;
         const int tile = HV_CROSS_FEW_ROWS(p.D);
         a.blocks = (p.Lq + tile - 1) / tile;
         const long lists = (long)p.B * (p.heads / 4), fit = 256L * (p.D == 40 ? 3 : 2);
@@ -527,17 +708,19 @@ static inline int hv_cross_attention_plan(const hv_cross_attention_params& p, Hv
         a.groups = (a.blocks + a.per_wg - 1) / a.per_wg;
         units = lists * a.groups;
     } else {
-        a.qt = rows > 64 ? 2 : 1;
-        a.blocks = (int)((rows + 64 * a.qt - 1) / (64 * a.qt));
-        a.per_wg = 1;
+        a.kernel = rows <= 16 ? 1 : rows <= 64 ? 2 : 3;
+        const int block = a.kernel == 1 ? 16 : a.kernel == 2 ? 64 : 128, least = a.kernel == 1 ? 512 : 256;
+        a.blocks = (int)((rows + block - 1) / block);
         const long base = pairs * a.blocks;
-        if (base < 512 && p.Lk >= 256) {  // too few workgroups to fill the chip: cut the keys
-            const long want = (1024 + base - 1) / (base > 0 ? base : 1), most = p.Lk / 128;
+        if (base > 0 && base < 512 && p.Lk >= 2 * least) {  // too few workgroups to fill the chip: cut the keys
+            const long want = (512 + base - 1) / base, most = p.Lk / least;
             a.splits = (int)(want < most ? want : most);
-            if (a.splits < 1) a.splits = 1;
+            a.per = ((p.Lk + a.splits - 1) / a.splits + 127) / 128 * 128;
+            a.splits = (p.Lk + a.per - 1) / a.per;
         }
-        a.groups = a.blocks;
-        units = pairs * a.groups * a.splits;
+        const long all = base * a.splits;
+        a.run = (int)(all / 64 < 1 ? 1 : all / 64 < a.blocks ? all / 64 : a.blocks);  // at least 64 runs: 8 for each XCD
+        units = all;
     }
     if (units > 0x3fffffffL) return -1;
     a.units = (int)units;
@@ -550,9 +733,10 @@ static inline long hv_cross_attention_floats(const HvCrossArgs& a) {
 
 template <int D>
 static inline void hv_cross_attention_launch_d(const HvCrossArgs& a, hipStream_t stream) {
-    const dim3 grid((unsigned)((a.units + 7) / 8 * 8)), block(256);
+    const int turn = 8 * a.run;
+    const dim3 grid((unsigned)(((long)a.units + turn - 1) / turn * turn)), block(256);
     if constexpr (D <= 80) {
-        if (a.few) {
+        if (a.kernel == 0) {
             const int nt = a.p.Lk <= 32 ? 2 : a.p.Lk <= 64 ? 4 : a.p.Lk <= 80 ? 5 : 6;
             hv_note("hv_cross_attention_few_kernel<%d,%d> | B=%d Lq=%d Lk=%d heads=%d/%d", D, nt, a.p.B, a.p.Lq, a.p.Lk, a.p.heads, a.p.kv_heads);
             if (nt == 2) hv_launch(hv_cross_attention_few_kernel<D, 2>, grid, block, stream, a);
@@ -562,13 +746,14 @@ static inline void hv_cross_attention_launch_d(const HvCrossArgs& a, hipStream_t
             return;
         }
     }
-    hv_note("hv_cross_attention_kernel<%d,%d> | B=%d Lq=%d Lk=%d heads=%d/%d splits=%d", D, a.qt, a.p.B, a.p.Lq, a.p.Lk, a.p.heads,
-            a.p.kv_heads, a.splits);
-    if (a.qt == 2) hv_launch(hv_cross_attention_kernel<D, 2, 2>, grid, block, stream, a);
-    else hv_launch(hv_cross_attention_kernel<D, 1, 2>, grid, block, stream, a);
+    hv_note("hv_cross_attention_%s<%d> | B=%d Lq=%d Lk=%d heads=%d/%d ranges=%d", a.kernel == 1 ? "rows_kernel" : a.kernel == 2 ? "kernel<1>" : "kernel<2>",
+            D, a.p.B, a.p.Lq, a.p.Lk, a.p.heads, a.p.kv_heads, a.splits);
+    if (a.kernel == 1) hv_launch(hv_cross_attention_rows_kernel<D>, grid, block, stream, a);
+    else if (a.kernel == 2) hv_launch(hv_cross_attention_kernel<D, 1>, grid, block, stream, a);
+    else hv_launch(hv_cross_attention_kernel<D, 2>, grid, block, stream, a);
     if (a.splits > 1) {
         const long items = (long)a.p.B * a.p.kv_heads * a.rows;
-        hv_note("hv_cross_attention_join_kernel<%d> | rows=%ld splits=%d", D, items, a.splits);
+        hv_note("hv_cross_attention_join_kernel<%d> | rows=%ld ranges=%d", D, items, a.splits);
         hv_launch(hv_cross_attention_join_kernel<D>, dim3((unsigned)((items + 3) / 4)), block, stream, a);
     }
 }

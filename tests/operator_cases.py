@@ -317,7 +317,7 @@ def case_chain(cx, B, Lq, Lk, heads, D, cdim, seed=0):
 
 def case_command_list(cx):
     """recorded into a command list, a replay recomputes from what the buffers then hold"""
-    B, Lq, Lk, H, D = 2, 3, 300, 2, 40
+    B, Lq, Lk, H, D = 2, 3, 1100, 2, 40
     g = _gen(cx, 5)
     q, k, v = (_put(cx, torch.randn(B, n, H * D, generator=g).to(BF16)) for n in (Lq, Lk, Lk))
     o = torch.zeros_like(q)

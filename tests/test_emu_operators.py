@@ -30,8 +30,12 @@ def cx():
     (1, 33, 65, 2, 2, 64, "both", "plain"),
     (2, 20, 97, 2, 2, 128, "both", "shared"),    # two chunks of 64
     (1, 130, 130, 1, 1, 160, "mask", "fused"),
-    (2, 9, 257, 2, 2, 160, "len", "plain"),      # keys cut into ranges
+    (2, 9, 257, 2, 2, 160, "len", "plain"),      # at most 16 rows: each wave its own keys
     (2, 1, 530, 4, 1, 128, "both", "fused"),     # shared key head, one query
+    (3, 2, 1100, 1, 1, 40, "len", "plain"),      # the same, keys cut into ranges
+    (1, 5, 1300, 3, 1, 64, "mask", "wide"),      # three heads to a key head
+    (3, 20, 600, 1, 1, 80, "both", "fused"),     # ranges of a chunked row block
+    (2, 70, 640, 1, 1, 40, "len", "plain"),
     (3, 2, 0, 2, 2, 40, None, "plain"),          # no states at all
     (2, 1, 3, 4, 4, 40, "len", "plain"),         # four heads a workgroup, states in registers
     (1, 131, 77, 4, 4, 40, "mask", "wide"),      # several tiles, the last one ragged
