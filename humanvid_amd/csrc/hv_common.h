@@ -183,6 +183,12 @@ HV_DEV void hv_vm_wait() {}
 HV_DEV void hv_barrier_raw() { __syncthreads(); }
 #endif
 
+HV_DEV void hv_sched_fence() {  // the scheduler moves nothing across: keeps a software pipeline's registers bounded
+#ifndef HV_EMU
+    __builtin_amdgcn_sched_barrier(0);
+#endif
+}
+
 // ---- gfx950 cross-lane / transposing LDS primitives -----------------------------------------------------
 // hv_lds_tr4: ds_read_b64_tr_b16.  Every lane supplies the 8-byte aligned LDS address of 4 consecutive bf16; within each
 // 16-lane group the 16 x 4 values are transposed: lane t of the group receives element (t & 3) of the lanes 4e + (t >> 2),

@@ -330,63 +330,69 @@ HV_DEV HvCrossPart hv_cross_part(const HvCrossArgs& a) {
 // fp32, and the products by 2^((m - m') c) are rare after the first chunk.
 #define HV_CROSS_SLACK 8.0f
 
-// ---- any number of states: a workgroup's 64 QT rows go through the keys in chunks of 64, staged in LDS for all four waves, the next
-// chunk on its way in registers.
+// ---- any number of states: a workgroup's 64 QT rows go through the keys in chunks of CH, two LDS stages filled by LDS-DMA, one
+// barrier a chunk.  Rows of K and V lie in LDS as in memory (D values), their 16-byte pieces rotated by a function of the row
+// so that the 16 rows of an access lie in different banks (5, 8, 10, 16 or 20 pieces a row repeat the banks after 16, 2, 8, 1, 4 rows).
+// In a chunk with a mask, or behind the end, the rows that are not attended are zeroed first.
+template <int D>
+struct HvCrossChunk {
+    static constexpr int P8 = D / 8, CH = D >= 128 ? 32 : 64, T = P8 % 16 == 0 ? 4 : P8 % 8 == 0 ? 3 : P8 % 4 == 0 ? 2 : P8 % 2 == 0 ? 1 : 0;
+    static constexpr int TILE = CH * D * 2, STAGE = 2 * TILE;
+    HV_DEV static int rot(int row) { return (row >> (4 - T)) & ((1 << T) - 1); }
+    HV_DEV static int at(int row, int piece) {  // byte offset of a piece
+        const int slot = piece + rot(row);
+        return (row * P8 + (slot < P8 ? slot : slot - P8)) * 16;
+    }
+};
 template <int D, int QT>
 __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_attention_kernel(HvCrossArgs a) {
     using Geom = HvCrossGeom<D>;
-    constexpr int KS = Geom::KS, DT = Geom::DT, P8 = Geom::P8, CH = 64, KSTR = Geom::KSTR, VSTR = Geom::VSTR;
-    constexpr int NV = (CH * P8 + 255) / 256;  // 16-byte pieces of K (and of V) that a thread stages
-    __shared__ __attribute__((aligned(16))) unsigned char sK[CH * KSTR];
-    __shared__ __attribute__((aligned(16))) unsigned char sV[CH * VSTR];
-    __shared__ __attribute__((aligned(16))) float sBias[CH];
+    using Chunk = HvCrossChunk<D>;
+    constexpr int KS = Geom::KS, DT = Geom::DT, P8 = Geom::P8, CH = Chunk::CH, KT = CH / 16;
+    constexpr int CI = CH * P8 / 64, NI = (2 * CI + 3) / 4;  // copy instructions of a K or V tile; of both, per wave
+    static_assert(CH * P8 % 64 == 0, "whole copy instructions");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * Chunk::STAGE];
+    __shared__ __attribute__((aligned(16))) float sBias[3][CH];  // zeros, and one for each stage
     const HvCrossPart part = hv_cross_part(a);
     if (part.none) return;
     const hv_cross_attention_params& p = a.p;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
-    const int b = part.b, kvh = part.kvh, k_end = part.end;
-    const int chunks = (k_end - part.begin + CH - 1) / CH;
-    const bf16_t* Kb = p.K + (long)b * p.k_stride_b + (long)kvh * D;
-    const bf16_t* Vb = p.V + (long)b * p.v_stride_b + (long)kvh * D;
-    const uint8_t* mask = p.key_mask ? p.key_mask + (long)b * p.mask_stride_b : nullptr;
-
-    // the zero columns D .. 32 KS of K and D .. 16 DT of V: written once, staging leaves them alone
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+#ifndef HV_EMU
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#else
+    const int wave = tid >> 6;
+#endif
+    const int b = part.b, kvh = part.kvh;
+    const int chunks = (part.end - part.begin + CH - 1) / CH;
+    const bf16_t* const Kb = p.K + (long)b * p.k_stride_b + (long)kvh * D;
+    const bf16_t* const Vb = p.V + (long)b * p.v_stride_b + (long)kvh * D;
+    const uint8_t* const mask = p.key_mask ? p.key_mask + (long)b * p.mask_stride_b : nullptr;
     const u32x4 zero4 = {0u, 0u, 0u, 0u};
-    if constexpr (KS * 4 > P8) {
-        for (int i = tid; i < CH * (KS * 4 - P8); i += 256)
-            hv_st16(sK + (i / (KS * 4 - P8)) * KSTR + (P8 + i % (KS * 4 - P8)) * 16, zero4);
-    }
-    if constexpr (DT * 2 > P8) {
-        for (int i = tid; i < CH; i += 256) hv_st16(sV + i * VSTR + P8 * 16, zero4);
-    }
 
-    u32x4 kreg[NV], vreg[NV];
-    float breg = 0.f;
-    auto fetch = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int idx = tid + i * 256, row = k0 + idx / P8, piece = idx % P8;
-            const bool on = idx < CH * P8 && row < k_end && (mask == nullptr || mask[row] != 0);
-            kreg[i] = on ? hv_ld16(Kb + (long)row * p.ldk + piece * 8) : zero4;
-            vreg[i] = on ? hv_ld16(Vb + (long)row * p.ldv + piece * 8) : zero4;
-        }
-        if (tid < CH) {
-            const int row = k0 + tid;
-            breg = row < k_end && (mask == nullptr || mask[row] != 0) ? 0.f : -INFINITY;
-        }
+    // copy instruction j = wave + 4 i: pieces 64 j .. of the K tile, behind CI those of the V tile
+    auto offset = [&](int j, int last) {
+        const int idx = (j < CI ? j : j - CI) * 64 + lane, row = idx / P8, slot = idx % P8;
+        int piece = slot - Chunk::rot(row);
+        piece = piece < 0 ? piece + P8 : piece;
+        return (unsigned)min(row, last) * (unsigned)((j < CI ? p.ldk : p.ldv) * 2) + (unsigned)(piece * 16);
     };
-    auto stage = [&]() {
+    unsigned ofs[NI];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int idx = tid + i * 256;
-            if (idx < CH * P8) {
-                hv_st16(sK + (idx / P8) * KSTR + (idx % P8) * 16, kreg[i]);
-                hv_st16(sV + (idx / P8) * VSTR + (idx % P8) * 16, vreg[i]);
-            }
+    for (int i = 0; i < NI; ++i) ofs[i] = offset(wave + 4 * i, CH);
+    uint8_t keep_next = 1;  // this lane's key of the next chunk
+    auto issue = [&](int ch, unsigned char* stage) {
+        const int k0 = part.begin + ch * CH, last = part.end - 1 - k0;
+        const char* const kb = (const char*)(Kb + (long)k0 * p.ldk);
+        const char* const vb = (const char*)(Vb + (long)k0 * p.ldv);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int j = wave + 4 * i;
+            if (j < 2 * CI) hv_glds16_s(j < CI ? kb : vb, last >= CH - 1 ? ofs[i] : offset(j, last), stage + j * 1024);
         }
-        if (tid < CH) sBias[tid] = breg;
+        if (mask != nullptr) keep_next = lane <= last && lane < CH ? mask[k0 + lane] : 0;
     };
-    fetch(part.begin);
+    if (chunks > 0) issue(0, smem);
+    if (tid < CH) sBias[0][tid] = 0.f;
 
     const int r0 = (part.block * 4 + wave) * QT * 16 + col;
     bf16x8 qf[QT][KS];
@@ -400,6 +406,13 @@ __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_atte
         for (int ks = 0; ks < KS; ++ks)
             qf[t][ks] = hv_as_bf16x8(r < a.rows && ks * 32 + g * 8 < D ? hv_ld16(src + ks * 32 + g * 8) : zero4);
     }
+    int kat[KS], vat[(DT + 1) / 2];  // a lane's places in the K tile (its row col) and in the V tile (row 4 g + col / 4)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) kat[ks] = Chunk::at(col, ks * 4 + g);
+#pragma unroll
+    for (int d = 0; d < (DT + 1) / 2; ++d)
+        vat[d] = Chunk::TILE + (2 * d < Geom::PAIRED ? Chunk::at(g * 4 + col / 4, d * 4 + (col & 3)) : Chunk::at(g * 4 + col / 4, d * 4 + (col & 3) / 2) + (col & 1) * 8);
+
     f32x4 acc[QT][DT], lsum[QT];
     float m[QT], mc[QT];
 #pragma unroll
@@ -411,30 +424,60 @@ __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_atte
         for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     for (int ch = 0; ch < chunks; ++ch) {
-        if (ch > 0) __syncthreads();  // the readers of the previous chunk are done
-        stage();
-        __syncthreads();
-        if (ch + 1 < chunks) fetch(part.begin + (ch + 1) * CH);
-        f32x4 s[QT][4];
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-            const f32x4 bias = *reinterpret_cast<const f32x4*>(sBias + kt * 16 + g * 4);
-#pragma unroll
-            for (int t = 0; t < QT; ++t) s[t][kt] = bias;
+        unsigned char* const stage = smem + (ch & 1) * Chunk::STAGE;
+        const int n = part.end - part.begin - ch * CH;
+        hv_vm_wait<0>();
+        hv_barrier_raw();  // the chunk has landed, and nobody reads the other stage any more
+        const bool kept = keep_next != 0;
+        if (ch + 1 < chunks) issue(ch + 1, smem + ((ch + 1) & 1) * Chunk::STAGE);
+        const float* bias = sBias[0] + g * 4;  // zeros
+        if (mask != nullptr || n < CH) {
+            const unsigned long keep = hv_ballot(lane < CH && lane < n && kept);
+            for (int i = tid; i < 2 * CH * P8; i += 256) {  // (rows keep their place: any order of the pieces will do)
+                const int row = i % CH, piece = i / CH;
+                if (!(keep >> row & 1ul)) hv_st16(stage + (piece < P8 ? 0 : Chunk::TILE) + (row * P8 + (piece < P8 ? piece : piece - P8)) * 16, zero4);
+            }
+            bias = sBias[1 + (ch & 1)] + g * 4;
+            if (tid < CH) sBias[1 + (ch & 1)][tid] = keep >> tid & 1ul ? 0.f : -INFINITY;
+            hv_barrier_raw();
+        }
+        f32x4 s[QT][KT];
+        u32x4 kv[2][KS];  // the next 16 keys' operands are read while this 16's are used; fences keep it at that
+        auto read_k = [&](int kt) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const bf16x8 kf = hv_as_bf16x8(hv_ld16(sK + (kt * 16 + col) * KSTR + ks * 64 + g * 16));
-#pragma unroll
-                for (int t = 0; t < QT; ++t) s[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][ks], s[t][kt], 0, 0, 0);
+                kv[kt & 1][ks] = zero4;
+                if ((ks + 1) * 32 <= D || ks * 32 + g * 8 < D) kv[kt & 1][ks] = hv_ld16(stage + kat[ks] + kt * (16 * P8 * 16));
             }
+        };
+        read_k(0);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            if (kt + 1 < KT) read_k(kt + 1);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) s[t][kt] = *reinterpret_cast<const f32x4*>(bias + kt * 16);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+                    s[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_as_bf16x8(kv[kt & 1][ks]), qf[t][ks], s[t][kt], 0, 0, 0);
+            hv_sched_fence();
         }
+        bf16x4 v0[2], v1[2];  // V fragments, one output tile ahead
+        auto read_v = [&](int i) {
+            const int pr = i / DT, d = i % DT;
+            const unsigned char* src = stage + vat[d / 2] + (d < Geom::PAIRED ? (d & 1) * 8 : 0) + pr * (32 * P8 * 16);
+            v0[i & 1] = hv_lds_tr4(src);
+            v1[i & 1] = hv_lds_tr4(src + 16 * P8 * 16);
+        };
+        read_v(0);
         float top[QT];
         bool past = false;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             top[t] = -INFINITY;
 #pragma unroll
-            for (int kt = 0; kt < 4; ++kt) top[t] = hv_max5(top[t], s[t][kt]);
+            for (int kt = 0; kt < KT; ++kt) top[t] = hv_max5(top[t], s[t][kt]);
             top[t] = hv_max_quarters(top[t]);
             past = past || (top[t] - m[t]) * a.c > HV_CROSS_SLACK;
         }
@@ -455,7 +498,7 @@ __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_atte
             }
         }
 #pragma unroll
-        for (int pr = 0; pr < 2; ++pr) {
+        for (int pr = 0; pr < KT / 2; ++pr) {
             bf16x8 pf[QT];
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
@@ -466,11 +509,16 @@ __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_atte
             }
 #pragma unroll
             for (int t = 0; t < QT; ++t) lsum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_bf16_ones(), pf[t], lsum[t], 0, 0, 0);
+            hv_sched_fence();
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const bf16x8 vf = hv_cross_vfrag<D>(sV, pr * 32, d, col, g);
+                const int i = pr * DT + d;
+                if (i + 1 < DT * KT / 2) read_v(i + 1);
+                const bf16x4 x = v0[i & 1], y = v1[i & 1];
+                const bf16x8 vf = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
 #pragma unroll
                 for (int t = 0; t < QT; ++t) acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], acc[t][d], 0, 0, 0);
+                hv_sched_fence();
             }
         }
     }
@@ -770,6 +818,7 @@ static inline int hv_cross_attention_launch(const hv_cross_attention_params& p, 
     if (rc) return rc;
     if (!(p.scale > 0.f) || p.scale > 3.0e38f) return -1;
     if (p.B == 0 || p.Lq == 0) return 0;
+    if (p.ldk < 0 || p.ldv < 0 || p.ldk > (1L << 24) || p.ldv > (1L << 24)) return -1;  // 64 rows within 32-bit offsets
     const uint64_t addr = (uint64_t)p.Q | (uint64_t)p.K | (uint64_t)p.V | (uint64_t)p.O;
     const long strides = p.ldq | p.ldk | p.ldv | p.ldo | p.q_stride_b | p.k_stride_b | p.v_stride_b | p.o_stride_b;
     if ((addr & 15) != 0 || (strides & 7) != 0) return -1;

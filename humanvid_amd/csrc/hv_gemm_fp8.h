@@ -87,12 +87,6 @@ HV_DEV f32x4 hv_fp8_block_product(const HvFp8Frag<true>& a, const HvFp8Frag<true
     return c;
 }
 
-HV_DEV void hv_sched_fence() {  // the scheduler moves nothing across: keeps a software pipeline's registers bounded
-#ifndef HV_EMU
-    __builtin_amdgcn_sched_barrier(0);
-#endif
-}
-
 struct HvGemmFp8Args {
     hv_gemm_fp8_params p;
     int kb;               // blocks of the reduction
