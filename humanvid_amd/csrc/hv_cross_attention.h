@@ -69,6 +69,12 @@ HV_DEV void hv_cross_row(const HvCrossArgs& a, int r, int kvh, int& query, int& 
     }
 }
 
+// workspace of a call whose keys are cut into ranges: per (batch, key head, row, range) D unnormalised sums, and behind all of those
+// the maximum and the sum of weights they refer to
+HV_DEV float* hv_cross_weights(const HvCrossArgs& a) {
+    return a.p.workspace + (long)a.p.B * a.p.kv_heads * a.rows * a.splits * a.p.D;
+}
+
 // geometry of the LDS copies and of a lane's share of the output for head dim D
 template <int D>
 struct HvCrossGeom {
@@ -456,11 +462,13 @@ __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_atte
             if (kt + 1 < KT) read_k(kt + 1);
 #pragma unroll
             for (int t = 0; t < QT; ++t) s[t][kt] = *reinterpret_cast<const f32x4*>(bias + kt * 16);
+            if (kt < 2 || n > 32) {  // (a last chunk of at most 32 keys leaves its second half out)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
+                for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                for (int t = 0; t < QT; ++t)
-                    s[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_as_bf16x8(kv[kt & 1][ks]), qf[t][ks], s[t][kt], 0, 0, 0);
+                    for (int t = 0; t < QT; ++t)
+                        s[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_as_bf16x8(kv[kt & 1][ks]), qf[t][ks], s[t][kt], 0, 0, 0);
+            }
             hv_sched_fence();
         }
         bf16x4 v0[2], v1[2];  // V fragments, one output tile ahead
@@ -499,6 +507,7 @@ __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_atte
         }
 #pragma unroll
         for (int pr = 0; pr < KT / 2; ++pr) {
+            if (pr > 0 && n <= 32) break;
             bf16x8 pf[QT];
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
@@ -527,19 +536,13 @@ __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_atte
         const int r = r0 + t * 16;
         if (r >= a.rows) continue;
         if (a.splits > 1) {  // unnormalised sums, with the maximum and the sum of weights they refer to
-            float* dst = p.workspace + ((((long)b * p.kv_heads + kvh) * a.rows + r) * a.splits + part.split) * (D + 2);
+            const long at = (((long)b * p.kv_heads + kvh) * a.rows + r) * a.splits + part.split;
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const int at = d < Geom::PAIRED ? d / 2 * 32 + g * 8 + (d & 1) * 4 : d * 16 + g * 4;
-                if (at < D) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) dst[2 + at + e] = acc[t][d][e];
-                }
+                const int c = d < Geom::PAIRED ? d / 2 * 32 + g * 8 + (d & 1) * 4 : d * 16 + g * 4;
+                if (c < D) *reinterpret_cast<f32x4*>(p.workspace + at * D + c) = acc[t][d];
             }
-            if (g == 0) {
-                dst[0] = m[t];
-                dst[1] = lsum[t][0];
-            }
+            if (g == 0) *reinterpret_cast<f32x2*>(hv_cross_weights(a) + at * 2) = f32x2{m[t], lsum[t][0]};
         } else {
             int query, column;
             hv_cross_row(a, r, kvh, query, column);
@@ -681,12 +684,9 @@ __global__ __launch_bounds__(256, 2) void hv_cross_attention_rows_kernel(HvCross
             o += x * q[2 + d];
         }
         if (a.splits > 1) {
-            float* dst = p.workspace + ((((long)b * p.kv_heads + kvh) * a.rows + r) * a.splits + part.split) * (D + 2);
-            dst[2 + d] = o;
-            if (d == 0) {
-                dst[0] = top;
-                dst[1] = l;
-            }
+            const long at = (((long)b * p.kv_heads + kvh) * a.rows + r) * a.splits + part.split;
+            p.workspace[at * D + d] = o;
+            if (d == 0) *reinterpret_cast<f32x2*>(hv_cross_weights(a) + at * 2) = f32x2{top, l};
         } else {
             int query, column;
             hv_cross_row(a, r, kvh, query, column);
@@ -695,40 +695,36 @@ __global__ __launch_bounds__(256, 2) void hv_cross_attention_rows_kernel(HvCross
     }
 }
 
-// joins the ranges of a row: o = sum_s o_s 2^((m_s - m) c) / sum_s l_s 2^((m_s - m) c); one wavefront per row
+// joins the ranges of a row: o = sum_s o_s 2^((m_s - m) c) / sum_s l_s 2^((m_s - m) c); four values of a row per thread
 template <int D>
 __global__ __launch_bounds__(256) void hv_cross_attention_join_kernel(HvCrossArgs a) {
     const hv_cross_attention_params& p = a.p;
-    const int lane = threadIdx.x & 63;
-    const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long i = (long)blockIdx.x * 256 + threadIdx.x, item = i / (D / 4);
+    const int d = (int)(i - item * (D / 4)) * 4;
     if (item >= (long)p.B * p.kv_heads * a.rows) return;
     const int r = (int)(item % a.rows);
     const int kvh = (int)(item / a.rows % p.kv_heads), b = (int)(item / a.rows / p.kv_heads);
-    const float* src = p.workspace + item * a.splits * (D + 2);
     int len = p.kv_len ? p.kv_len[b] : p.Lk;
     len = len > p.Lk ? p.Lk : len;
     const int ranges = len <= a.per ? 1 : (len + a.per - 1) / a.per;  // those behind the entry's end wrote nothing
+    const f32x2* const ml = reinterpret_cast<const f32x2*>(hv_cross_weights(a)) + item * a.splits;
+    const float* const src = p.workspace + item * a.splits * D + d;
     float m = -INFINITY;
-    for (int s = 0; s < ranges; ++s) m = hv_max(m, src[s * (D + 2)]);
+    for (int s = 0; s < ranges; ++s) m = hv_max(m, ml[s][0]);
     const float ms = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[(D + 63) / 64];
-#pragma unroll
-    for (int i = 0; i < (D + 63) / 64; ++i) o[i] = 0.f;
+    float l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < ranges; ++s) {
-        const float* q = src + s * (D + 2);
-        const float w = __builtin_amdgcn_exp2f((q[0] - ms) * a.c);
-        l += w * q[1];
+        const float w = __builtin_amdgcn_exp2f((ml[s][0] - ms) * a.c);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(src + (long)s * D);
+        l += w * ml[s][1];
 #pragma unroll
-        for (int i = 0; i < (D + 63) / 64; ++i)
-            if (i * 64 + lane < D) o[i] += w * q[2 + i * 64 + lane];
+        for (int e = 0; e < 4; ++e) o[e] += w * v[e];
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     int query, column;
     hv_cross_row(a, r, kvh, query, column);
-    bf16_t* dst = p.O + (long)b * p.o_stride_b + (long)query * p.ldo + column;
-#pragma unroll
-    for (int i = 0; i < (D + 63) / 64; ++i)
-        if (i * 64 + lane < D) dst[i * 64 + lane] = hv_f2bf(o[i] * inv);
+    hv_st8(p.O + (long)b * p.o_stride_b + (long)query * p.ldo + column + d, u32x2{hv_pack2(o[0] * inv, o[1] * inv), hv_pack2(o[2] * inv, o[3] * inv)});
 }
 
 // sizes -> how the work is cut (also what hv_cross_attention_workspace answers from): -1 invalid, -2 head dim
@@ -760,8 +756,10 @@ static inline int hv_cross_attention_plan(const hv_cross_attention_params& p, Hv
         const int block = a.kernel == 1 ? 16 : a.kernel == 2 ? 64 : 128, least = a.kernel == 1 ? 512 : 256;
         a.blocks = (int)((rows + block - 1) / block);
         const long base = pairs * a.blocks;
-        if (base > 0 && base < 512 && p.Lk >= 2 * least) {  // too few workgroups to fill the chip: cut the keys
-            const long want = (512 + base - 1) / base, most = p.Lk / least;
+        if (base > 0 && base < 512 && p.Lk >= 2 * least) {
+            // too few workgroups to fill the chip: cut the keys, to twice as many workgroups where entries may be of different lengths
+            // (4 x 1536 queries, up to 4109 states, D = 80: ragged 80 us against 97, all full 114 against 104)
+            const long want = ((p.kv_len ? 1024 : 512) + base - 1) / base, most = p.Lk / least;
             a.splits = (int)(want < most ? want : most);
             a.per = ((p.Lk + a.splits - 1) / a.splits + 127) / 128 * 128;
             a.splits = (p.Lk + a.per - 1) / a.per;
@@ -802,7 +800,7 @@ static inline void hv_cross_attention_launch_d(const HvCrossArgs& a, hipStream_t
     if (a.splits > 1) {
         const long items = (long)a.p.B * a.p.kv_heads * a.rows;
         hv_note("hv_cross_attention_join_kernel<%d> | rows=%ld ranges=%d", D, items, a.splits);
-        hv_launch(hv_cross_attention_join_kernel<D>, dim3((unsigned)((items + 3) / 4)), block, stream, a);
+        hv_launch(hv_cross_attention_join_kernel<D>, dim3((unsigned)((items * (D / 4) + 255) / 256)), block, stream, a);
     }
 }
 
@@ -822,7 +820,7 @@ static inline int hv_cross_attention_launch(const hv_cross_attention_params& p, 
     const uint64_t addr = (uint64_t)p.Q | (uint64_t)p.K | (uint64_t)p.V | (uint64_t)p.O;
     const long strides = p.ldq | p.ldk | p.ldv | p.ldo | p.q_stride_b | p.k_stride_b | p.v_stride_b | p.o_stride_b;
     if ((addr & 15) != 0 || (strides & 7) != 0) return -1;
-    if (hv_cross_attention_floats(a) > p.workspace_floats || (a.splits > 1 && (p.workspace == nullptr || ((uint64_t)p.workspace & 3) != 0))) return -3;
+    if (hv_cross_attention_floats(a) > p.workspace_floats || (a.splits > 1 && (p.workspace == nullptr || ((uint64_t)p.workspace & 15) != 0))) return -3;
     switch (p.D) {
         case 40: hv_cross_attention_launch_d<40>(a, stream); break;
         case 64: hv_cross_attention_launch_d<64>(a, stream); break;
