@@ -6,8 +6,8 @@
 // A block of 128 is exactly one v_mfma_f32_16x16x128_f8f6f4: every instruction starts from a zero accumulator and its four
 // results per lane are added to the fp32 sums with the block's factor xs ws -- 4 v_fma per 32-cycle MFMA, which fit under it.
 // The operands are taken as A = W (rows n), B = X (columns m): a lane then owns ONE row m of Y per 16-row tile, so xs is one
-// value per lane and tile, and the four W tiles of a 64-column block are read from LDS in an order that leaves the lane 16
-// consecutive columns (n = 16 (lane >> 4) + 4 t + r): 16-byte stores, whole 128-byte lines per wave.
+// value per lane and tile, and the four W tiles of a 64-column block are read from LDS in an order that leaves the lane twice
+// 8 consecutive columns: 16-byte stores, the four lanes of a row 64 bytes in one.
 // Both operands are read with the same lane -> k assignment, so its order inside a block does not matter to the sum.
 //
 // Precision: the 8-bit matrix instructions (16x16x128 and 16x16x32 alike) add the products of 8 neighbouring k after aligning them
@@ -94,51 +94,55 @@ struct HvGemmFp8Args {
     int vec;              // Y and the residual take 16-byte accesses
 };
 
-// 16 consecutive columns n .. n + 15 of row m: bias, residual, rounding, store
+// 8 consecutive columns n .. n + 7 of row m: residual, rounding, store
 HV_DEV void hv_gemm_fp8_store(const HvGemmFp8Args& a, int m, int n, float* v) {
     const hv_gemm_fp8_params& p = a.p;
-    if (a.vec && n + 16 <= p.N) {
+    if (a.vec && n + 8 <= p.N) {
         if (p.residual) {
-            const bf16_t* r = p.residual + (long)m * p.ldr + n;
-            float f[16];
-            hv_unpack8(hv_ld16(r), f);
-            hv_unpack8(hv_ld16(r + 8), f + 8);
+            float f[8];
+            hv_unpack8(hv_ld16(p.residual + (long)m * p.ldr + n), f);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] += f[i];
+            for (int i = 0; i < 8; ++i) v[i] += f[i];
         }
         if (p.out_f32) {
             float* y = (float*)p.Y + (long)m * p.ldy + n;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4*>(y + 4 * i) = f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+            *reinterpret_cast<f32x4*>(y) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4*>(y + 4) = f32x4{v[4], v[5], v[6], v[7]};
         } else {
-            bf16_t* y = (bf16_t*)p.Y + (long)m * p.ldy + n;
-            hv_st16(y, hv_pack8(v));
-            hv_st16(y + 8, hv_pack8(v + 8));
+            hv_st16((bf16_t*)p.Y + (long)m * p.ldy + n, hv_pack8(v));
         }
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        if (n + i >= p.N) break;
-        float x = v[i];
-        if (p.residual) x += hv_bf2f(p.residual[(long)m * p.ldr + n + i]);
-        if (p.out_f32) ((float*)p.Y)[(long)m * p.ldy + n + i] = x;
-        else ((bf16_t*)p.Y)[(long)m * p.ldy + n + i] = hv_f2bf(x);
+    for (int i = 0; i < 8; ++i) {
+        if (n + i < p.N) {
+            float x = v[i];
+            if (p.residual) x += hv_bf2f(p.residual[(long)m * p.ldr + n + i]);
+            if (p.out_f32) ((float*)p.Y)[(long)m * p.ldy + n + i] = x;
+            else ((bf16_t*)p.Y)[(long)m * p.ldy + n + i] = hv_f2bf(x);
+        }
     }
 }
 
 // ---- tiles: WM x WN waves, a wave computes 16 MT rows x 64 columns; two LDS stages of one 128-block each, filled by LDS-DMA.
 // LDS rows are 128 bytes (one block), their 16-byte pieces XOR-swizzled on the source side: X by (row >> 1) & 7; W, whose 16
-// rows of an MFMA are {16 q + 4 t + r}, by (row >> 1 & 1) | (row >> 4 & 3) << 1 -- both leave the 16 lanes of a ds_read_b128 on
-// 16 different quarters of the 64 banks.  The pieces behind K in the last block hold repeated values of the same row; their X
-// side is zeroed in registers.
+// rows of an MFMA are 32 (i / 2) + 8 q + 4 (i & 1) + r, by (row >> 1 & 1) | (row >> 3 & 3) << 1 -- both leave the 16 lanes of a
+// ds_read_b128 on 16 different quarters of the 64 banks.  The pieces behind K in the last block hold repeated values of the same row;
+// their X side is zeroed in LDS.
+// Workgroups are persistent: the first block of the next tile is on its way while the last one of this tile is computed and its
+// results are stored -- one workgroup fills a CU's registers and LDS, so nothing else would cover that (147456 x 960 x 320: 131 -> 124 us;
+// 18432 x 10240 x 1280: 309 -> 306).
+// What bounds it: per block and wave 32 MFMAs (1024 cycles) and 128 fused multiply-adds for the block's scales (4 cycles each, which the
+// matrix pipe does not hide), twice that per SIMD, of 5800 measured: 0.77 of what the two take one after the other; short
+// reductions by the stores (283 MB of the 330 MB at K = 320).
 template <int WM, int WN, int MT, bool WIDE>
 __global__ __launch_bounds__(64 * WM * WN, 2) void hv_gemm_fp8_kernel(HvGemmFp8Args a) {
     constexpr int BM = WM * MT * 16, BN = WN * 64, WAVES = WM * WN;
     constexpr int XB = BM * 128, WB = BN * 128, SB = BM * 4;       // bytes of a stage: X, W, the rows' scales
     constexpr int XI = XB / 1024 / WAVES, WI = WB / 1024 / WAVES;  // DMA instructions (1024 bytes) per wave and stage
-    static_assert(XI * WAVES * 1024 == XB && WI * WAVES * 1024 == WB && BM / 64 <= WAVES, "whole instructions per wave");
+    static_assert(XI * WAVES * 1024 == XB && WI * WAVES * 1024 == WB && BM / 64 <= WAVES && WAVES % 4 == 0, "whole instructions per wave");
     __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * (XB + WB + SB)];
+    __shared__ __attribute__((aligned(1024))) float sBias[2][BN];  // this tile's and the next one's
     const hv_gemm_fp8_params& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
 #ifndef HV_EMU
@@ -148,113 +152,154 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void hv_gemm_fp8_kernel(HvGemmFp8A
 #endif
     const int wm = wave % WM, wn = wave / WM;
 
-    // an XCD takes a contiguous range of tiles; inside it groups of 8 row tiles, the row tiles of a column tile adjacent: the
-    // 32 tiles in flight share 8 panels of X and 4 of W in its L2
-    const int total = a.tiles_m * a.tiles_n, per_xcd = (total + 7) / 8;
-    const int t = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per_xcd || t >= total) return;
-    const int grp = t / (8 * a.tiles_n), in_grp = t % (8 * a.tiles_n);
-    const int gm = min(8, a.tiles_m - grp * 8);
-    const int m0 = (grp * 8 + in_grp % gm) * BM, n0 = in_grp / gm * BN;
+    // an XCD takes a contiguous range of tiles, its workgroups the next ones in turn; inside it groups of 8 row tiles, the row tiles of a
+    // column tile adjacent: the 32 tiles in flight share 8 panels of X and 4 of W in its L2
+    const int total = a.tiles_m * a.tiles_n, per_xcd = (total + 7) / 8, turn = gridDim.x / 8;
+    const int t_end = min(((int)(blockIdx.x & 7) + 1) * per_xcd, total);
+    int t = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+    if (t >= t_end) return;
 
     // DMA sources: instruction I = wave + WAVES i of a tile carries rows 8 I .. 8 I + 7, lane l the piece (l & 7) ^ key(row) of row
-    // 8 I + l / 8; I has the same parity for every i and, with 4 waves, I / 2 one of two values mod 4.  Rows past the end repeat
-    // the last row (their products are never stored).
-    const char* const xbase = (const char*)p.X + (long)m0 * p.ldx;
-    const char* const wbase = (const char*)p.W + (long)n0 * p.ldw;
-    const char* const sbase = (const char*)(p.x_scale + (long)m0 * p.x_scale_row);
+    // 8 I + l / 8; WAVES is a multiple of 4, so a lane's piece is the same for every i.  Rows past the end repeat the last row (their
+    // products are never stored).
     const int xpiece = ((lane & 7) ^ ((4 * (wave & 1) + (lane >> 4)) & 7)) * 16;
-    const int wpiece = ((lane & 7) ^ (((lane >> 4) & 1) | (((wave >> 1) & 3) << 1))) * 16;  // i odd, 4 waves: ^ (2 << 1) * 16
+    const int wpiece = ((lane & 7) ^ (((lane >> 4) & 1) | ((wave & 3) << 1))) * 16;
+    int m0 = 0, n0 = 0;
+    const char *xbase = nullptr, *wbase = nullptr, *sbase = nullptr;
+    const float* wsp = nullptr;
     unsigned xofs[XI], wofs[WI], sofs = 0;
+    auto place = [&](int tile) {
+        const int grp = tile / (8 * a.tiles_n), in_grp = tile % (8 * a.tiles_n), gm = min(8, a.tiles_m - grp * 8);
+        m0 = (grp * 8 + in_grp % gm) * BM;
+        n0 = in_grp / gm * BN;
+        xbase = (const char*)p.X + (long)m0 * p.ldx;
+        wbase = (const char*)p.W + (long)n0 * p.ldw;
+        sbase = (const char*)(p.x_scale + (long)m0 * p.x_scale_row);
+        wsp = p.w_scale + (long)(min(n0 + wn * 64, p.N - 1) / 128) * p.w_scale_row;
 #pragma unroll
-    for (int i = 0; i < XI; ++i) xofs[i] = (unsigned)min((wave + WAVES * i) * 8 + (lane >> 3), p.M - 1 - m0) * (unsigned)p.ldx;
+        for (int i = 0; i < XI; ++i) xofs[i] = (unsigned)min((wave + WAVES * i) * 8 + (lane >> 3), p.M - 1 - m0) * (unsigned)p.ldx;
 #pragma unroll
-    for (int i = 0; i < WI; ++i) wofs[i] = (unsigned)min((wave + WAVES * i) * 8 + (lane >> 3), p.N - 1 - n0) * (unsigned)p.ldw;
-    if (wave < BM / 64) sofs = (unsigned)min(tid, p.M - 1 - m0) * (unsigned)(p.x_scale_row * 4);
+        for (int i = 0; i < WI; ++i) wofs[i] = (unsigned)min((wave + WAVES * i) * 8 + (lane >> 3), p.N - 1 - n0) * (unsigned)p.ldw;
+        if (wave < BM / 64) sofs = (unsigned)min(tid, p.M - 1 - m0) * (unsigned)(p.x_scale_row * 4);
+    };
+    float wnext = 0.f;
     auto issue = [&](int kb, int st) {
         unsigned char* xs = smem + st * (XB + WB + SB);
         unsigned char* ws = xs + XB;
         const int left = p.K - kb * 128 - 16;  // last piece inside K
-        const unsigned xp = (unsigned)min(xpiece, left);
-        const unsigned wp[2] = {(unsigned)min(wpiece, left), (unsigned)min(WAVES == 4 ? wpiece ^ 64 : wpiece, left)};
+        const unsigned xp = (unsigned)min(xpiece, left), wp = (unsigned)min(wpiece, left);
+        wnext = wsp[(long)kb * p.w_scale_k];
 #pragma unroll
         for (int i = 0; i < XI; ++i) hv_glds16_s(xbase + (long)kb * 128, xofs[i] + xp, xs + (wave + WAVES * i) * 1024);
 #pragma unroll
-        for (int i = 0; i < WI; ++i) hv_glds16_s(wbase + (long)kb * 128, wofs[i] + wp[i & 1], ws + (wave + WAVES * i) * 1024);
+        for (int i = 0; i < WI; ++i) hv_glds16_s(wbase + (long)kb * 128, wofs[i] + wp, ws + (wave + WAVES * i) * 1024);
         if (wave < BM / 64) hv_glds4_s(sbase + (long)kb * p.x_scale_k * 4, sofs, ws + WB + wave * 256);
     };
+    auto issue_bias = [&](int which) {
+        if (p.bias != nullptr && wave < BN / 64) hv_glds4_s(p.bias + n0, (unsigned)min(tid, p.N - 1 - n0) * 4u, &sBias[which][wave * 64]);
+    };
 
-    const float* wsp = p.w_scale + (long)(min(n0 + wn * 64, p.N - 1) / 128) * p.w_scale_row;
-    f32x4 acc[4][MT];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
+    place(t);
     issue(0, 0);
-    float wnext = wsp[0];
-    for (int kb = 0; kb < a.kb; ++kb) {
-        const int st = kb & 1;
-        const float wsc = wnext;
-        hv_vm_wait<0>();
-        hv_barrier_raw();  // block kb has landed, and nobody reads the other stage any more
-        if (kb + 1 < a.kb) {
-            issue(kb + 1, st ^ 1);
-            wnext = wsp[(long)(kb + 1) * p.w_scale_k];
-        }
-        unsigned char* xs = smem + st * (XB + WB + SB);
-        const unsigned char* ws = xs + XB;
-        const float* ss = reinterpret_cast<const float*>(ws + WB) + wm * MT * 16 + col;
-        const int left = p.K - kb * 128;
-        if (left < 128) {  // the last block is short: X is zero behind K
-            for (int i = tid; i < BM * 8; i += 64 * WAVES) {
-                const int row = i >> 3;
-                if ((i & 7) * 16 >= left) hv_st16(xs + row * 128 + (((i & 7) ^ ((row >> 1) & 7)) << 4), u32x4{0u, 0u, 0u, 0u});
+    issue_bias(0);
+    bool stores = false;  // the last tile's 2 MT stores, and nothing else, are younger than the copies in flight
+    for (int st = 0, odd = 0;; odd ^= 1) {
+        const int mt = m0, nt = n0;  // this tile
+        const int next = t + turn;
+        f32x4 acc[4][MT];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int kb = 0; kb < a.kb; ++kb, st ^= 1) {
+            if (kb == 0 && stores) hv_vm_wait<2 * MT>();
+            else hv_vm_wait<0>();
+            hv_barrier_raw();  // block kb has landed, and nobody reads the other stage any more
+            const float wsc = wnext;
+            if (kb + 1 < a.kb) {
+                issue(kb + 1, st ^ 1);
+            } else if (next < t_end) {
+                place(next);
+                issue(0, st ^ 1);
+                issue_bias(odd ^ 1);
             }
-            __syncthreads();
-        }
-        // fragments: row 16 j + col of the wave's X rows, key (col >> 1); row 16 (col / 4) + 4 i + col % 4 of its W rows
-        const unsigned char* const xrow = xs + (wm * MT * 16 + col) * 128;
-        const unsigned char* const wrow = ws + (wn * 64 + (col >> 2) * 16 + (col & 3)) * 128;
-        const int xk = (g ^ (col >> 1)) << 4, wk = (g ^ (((col >> 1) & 1) | ((col >> 2) << 1))) << 4;  // the second piece: ^ 64
-        HvFp8Frag<WIDE> wf[4], xf[2];
-        f32x4 part[2][4];
-        float f[2];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) wf[i].set(hv_ld16(wrow + i * 512 + wk), hv_ld16(wrow + i * 512 + (wk ^ 64)));
-        xf[0].set(hv_ld16(xrow + xk), hv_ld16(xrow + (xk ^ 64)));
-        f[0] = ss[0] * wsc;
-        // row tile j's products are in flight while row tile j - 1's are added up
-#pragma unroll
-        for (int j = 0; j <= MT; ++j) {
-            if (j + 1 < MT) xf[(j + 1) & 1].set(hv_ld16(xrow + (j + 1) * 2048 + xk), hv_ld16(xrow + (j + 1) * 2048 + (xk ^ 64)));
-            if (j < MT) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) part[j & 1][i] = hv_fp8_block_product(wf[i], xf[j & 1]);
+            unsigned char* xs = smem + st * (XB + WB + SB);
+            const unsigned char* ws = xs + XB;
+            const float* ss = reinterpret_cast<const float*>(ws + WB) + wm * MT * 16 + col;
+            const int left = p.K - kb * 128;
+            if (left < 128) {  // the last block is short: X is zero behind K
+                for (int i = tid; i < BM * 8; i += 64 * WAVES) {
+                    const int row = i >> 3;
+                    if ((i & 7) * 16 >= left) hv_st16(xs + row * 128 + (((i & 7) ^ ((row >> 1) & 7)) << 4), u32x4{0u, 0u, 0u, 0u});
+                }
+                hv_barrier_raw();
             }
-            if (j > 0) {
+            // fragments: row 16 j + col of the wave's X rows, key (col >> 1); row 32 (i / 2) + 8 (col / 4) + 4 (i & 1) + col % 4 of its W rows
+            const unsigned char* const xrow = xs + (wm * MT * 16 + col) * 128;
+            const unsigned char* const wrow = ws + (wn * 64 + (col >> 2) * 8 + (col & 3)) * 128;
+            const int xk = (g ^ (col >> 1)) << 4, wk = (g ^ (((col >> 1) & 1) | ((col >> 2) << 1))) << 4;  // the second piece: ^ 64
+            HvFp8Frag<WIDE> wf[4], xf[2];
+            f32x4 part[2][4];
+            float f[2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) wf[i].set(hv_ld16(wrow + (i / 2) * 4096 + (i & 1) * 512 + wk), hv_ld16(wrow + (i / 2) * 4096 + (i & 1) * 512 + (wk ^ 64)));
+            xf[0].set(hv_ld16(xrow + xk), hv_ld16(xrow + (xk ^ 64)));
+            f[0] = ss[0] * wsc;
+            // row tile j's products are in flight while row tile j - 1's are added up
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[i][j - 1][r] = fmaf(part[(j - 1) & 1][i][r], f[(j - 1) & 1], acc[i][j - 1][r]);
+            for (int j = 0; j <= MT; ++j) {
+                if (j + 1 < MT) xf[(j + 1) & 1].set(hv_ld16(xrow + (j + 1) * 2048 + xk), hv_ld16(xrow + (j + 1) * 2048 + (xk ^ 64)));
+                if (j < MT) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) part[j & 1][i] = hv_fp8_block_product(wf[i], xf[j & 1]);
+                }
+                if (j > 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[i][j - 1][r] = fmaf(part[(j - 1) & 1][i][r], f[(j - 1) & 1], acc[i][j - 1][r]);
+                }
+                if (j + 1 < MT) f[(j + 1) & 1] = ss[(j + 1) * 16] * wsc;
+                hv_sched_fence();
             }
-            if (j + 1 < MT) f[(j + 1) & 1] = ss[(j + 1) * 16] * wsc;
-            hv_sched_fence();
         }
-    }
 
-    const int n = n0 + wn * 64 + g * 16;
-    float bias[16];
+        // a lane's results of row tile j: row mt + 16 (wm MT + j) + col, columns n .. n + 7 and n + 32 .. n + 39
+        const int n = nt + wn * 64 + g * 8;
+        float bias[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) bias[i] = p.bias && n + i < p.N ? p.bias[n + i] : 0.f;
+        for (int i = 0; i < 16; i += 4) {
+            f32x4 b = {0.f, 0.f, 0.f, 0.f};
+            if (p.bias != nullptr) b = *reinterpret_cast<const f32x4*>(&sBias[odd][wn * 64 + g * 8 + (i / 8) * 32 + i % 8]);
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-        const int m = m0 + (wm * MT + j) * 16 + col;
-        if (m >= p.M || n >= p.N) continue;
-        float v[16];
+            for (int e = 0; e < 4; ++e) bias[i + e] = b[e];
+        }
+        stores = !WIDE && a.vec && p.residual == nullptr && mt + BM <= p.M && nt + BN <= p.N;
+        if (stores) {
+            bf16_t* y = (bf16_t*)p.Y + (long)(mt + wm * MT * 16 + col) * p.ldy + n;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = acc[i / 4][j][i % 4] + bias[i];
-        hv_gemm_fp8_store(a, m, n, v);
+            for (int j = 0; j < MT; ++j, y += 16 * p.ldy) {
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = acc[i / 4][j][i % 4] + bias[i];
+                hv_st16(y, hv_pack8(v));
+                hv_st16(y + 32, hv_pack8(v + 8));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                const int m = mt + (wm * MT + j) * 16 + col;
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = acc[i / 4][j][i % 4] + bias[i];
+                if (m < p.M) {
+                    hv_gemm_fp8_store(a, m, n, v);
+                    hv_gemm_fp8_store(a, m, n + 32, v + 8);
+                }
+            }
+        }
+        t = next;
+        if (t >= t_end) break;
     }
 }
 
@@ -345,23 +390,24 @@ static inline int hv_gemm_fp8_launch(const hv_gemm_fp8_params& p, hipStream_t st
         return 0;
     }
     auto tiles = [&](int bm, int bn) { return (long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
-    auto set = [&](int bm, int bn) {
+    auto set = [&](int bm, int bn, long fit) {  // fit: workgroups the chip holds at once
         a.tiles_m = (p.M + bm - 1) / bm;
         a.tiles_n = (p.N + bn - 1) / bn;
-        return dim3((unsigned)((tiles(bm, bn) + 7) / 8 * 8));
+        const long n = (tiles(bm, bn) + 7) / 8 * 8;
+        return dim3((unsigned)(n < fit ? n : fit));
     };
     if (tiles(64, 64) > 0x3fffffffL) return -1;
     if (!p.out_f32 && (g_hv_gemm_fp8_tile == 256 || (g_hv_gemm_fp8_tile == 0 && tiles(256, 256) >= 256))) {
-        const dim3 grid = set(256, 256);
+        const dim3 grid = set(256, 256, 256);
         hv_note("hv_gemm_fp8_kernel<2,4,8> | M=%d N=%d K=%d", p.M, p.N, p.K);
         hv_launch(hv_gemm_fp8_kernel<2, 4, 8, false>, grid, dim3(512), stream, a);
     } else if (g_hv_gemm_fp8_tile >= 128 || (g_hv_gemm_fp8_tile == 0 && tiles(128, 128) >= 256)) {
-        const dim3 grid = set(128, 128);
+        const dim3 grid = set(128, 128, 512);
         hv_note("hv_gemm_fp8_kernel<2,2,4> | M=%d N=%d K=%d", p.M, p.N, p.K);
         if (p.out_f32) hv_launch(hv_gemm_fp8_kernel<2, 2, 4, true>, grid, dim3(256), stream, a);
         else hv_launch(hv_gemm_fp8_kernel<2, 2, 4, false>, grid, dim3(256), stream, a);
     } else {
-        const dim3 grid = set(64, 64);
+        const dim3 grid = set(64, 64, 1024);
         hv_note("hv_gemm_fp8_kernel<4,1,1> | M=%d N=%d K=%d", p.M, p.N, p.K);
         if (p.out_f32) hv_launch(hv_gemm_fp8_kernel<4, 1, 1, true>, grid, dim3(256), stream, a);
         else hv_launch(hv_gemm_fp8_kernel<4, 1, 1, false>, grid, dim3(256), stream, a);
