@@ -709,17 +709,33 @@ __global__ __launch_bounds__(256) void hv_cross_attention_join_kernel(HvCrossArg
     const int ranges = len <= a.per ? 1 : (len + a.per - 1) / a.per;  // those behind the entry's end wrote nothing
     const f32x2* const ml = reinterpret_cast<const f32x2*>(hv_cross_weights(a)) + item * a.splits;
     const float* const src = p.workspace + item * a.splits * D + d;
-    float m = -INFINITY;
-    for (int s = 0; s < ranges; ++s) m = hv_max(m, ml[s][0]);
-    const float ms = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
+    float m = -INFINITY, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < ranges; ++s) {
-        const float w = __builtin_amdgcn_exp2f((ml[s][0] - ms) * a.c);
-        const f32x4 v = *reinterpret_cast<const f32x4*>(src + (long)s * D);
-        l += w * ml[s][1];
+    constexpr int U = 4;  // ranges whose loads are in flight together
+    for (int s0 = 0; s0 < ranges; s0 += U) {
+        f32x2 w[U];
+        f32x4 v[U];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += w * v[e];
+        for (int u = 0; u < U; ++u) {
+            const int s = min(s0 + u, ranges - 1);
+            w[u] = ml[s];
+            v[u] = *reinterpret_cast<const f32x4*>(src + (long)s * D);
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) top = hv_max(top, w[u][0]);
+        const float ms = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f((m - ms) * a.c);
+        m = top;
+        l *= old;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= old;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float x = s0 + u < ranges ? __builtin_amdgcn_exp2f((w[u][0] - ms) * a.c) : 0.f;
+            l += x * w[u][1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += x * v[u][e];
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     int query, column;

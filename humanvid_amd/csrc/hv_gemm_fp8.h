@@ -91,6 +91,7 @@ struct HvGemmFp8Args {
     hv_gemm_fp8_params p;
     int kb;               // blocks of the reduction
     int tiles_m, tiles_n;
+    int splits, per;      // ranges of the reduction (few tiles), blocks per range
     int vec;              // Y and the residual take 16-byte accesses
 };
 
@@ -303,8 +304,123 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void hv_gemm_fp8_kernel(HvGemmFp8A
     }
 }
 
+// ---- few tiles: 64 x 64 of them, four waves of 16 rows, where 128 x 128 tiles would not give every CU one.  What counts there is the
+// time a block of the reduction takes to arrive: four LDS stages, three blocks in flight, and with splits > 1 the blocks are divided among
+// workgroups whose fp32 sums the join kernel adds up (in order: the result does not depend on which came first).  Every wave issues
+// the same six copies a block (the scales four times over), so the waits can count them.
+template <bool WIDE>
+__global__ __launch_bounds__(256) void hv_gemm_fp8_small_kernel(HvGemmFp8Args a) {
+    constexpr int XB = 64 * 128, STAGE = 2 * XB, S = 4;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[S * STAGE];
+    __shared__ __attribute__((aligned(1024))) float sXs[S][64];
+    __shared__ __attribute__((aligned(1024))) float sWs[S][64];
+    const hv_gemm_fp8_params& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+#ifndef HV_EMU
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#else
+    const int wave = tid >> 6;
+#endif
+    const int total = a.tiles_m * a.tiles_n, tile = blockIdx.x % total, split = blockIdx.x / total;
+    const int m0 = tile % a.tiles_m * 64, n0 = tile / a.tiles_m * 64;
+    const int k_begin = split * a.per, k_end = min(k_begin + a.per, a.kb);
+    const char* const xbase = (const char*)p.X + (long)m0 * p.ldx;
+    const char* const wbase = (const char*)p.W + (long)n0 * p.ldw;
+    const int xpiece = ((lane & 7) ^ ((4 * (wave & 1) + (lane >> 4)) & 7)) * 16;  // the tile kernel's swizzles
+    const int wpiece = ((lane & 7) ^ (((lane >> 4) & 1) | ((wave & 3) << 1))) * 16;
+    unsigned xofs[2], wofs[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        xofs[i] = (unsigned)min((wave + 4 * i) * 8 + (lane >> 3), p.M - 1 - m0) * (unsigned)p.ldx;
+        wofs[i] = (unsigned)min((wave + 4 * i) * 8 + (lane >> 3), p.N - 1 - n0) * (unsigned)p.ldw;
+    }
+    const float* const sbase = p.x_scale + (long)m0 * p.x_scale_row;
+    const unsigned sofs = (unsigned)min(lane, p.M - 1 - m0) * (unsigned)(p.x_scale_row * 4);
+    const float* const wsp = p.w_scale + (long)(n0 / 128) * p.w_scale_row;  // 64 columns lie in one block of W's scales
+    auto issue = [&](int kb) {
+        const int st = kb & (S - 1);
+        unsigned char* xs = smem + st * STAGE;
+        const int left = p.K - kb * 128 - 16;
+        const unsigned xp = (unsigned)min(xpiece, left), wp = (unsigned)min(wpiece, left);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            hv_glds16_s(xbase + (long)kb * 128, xofs[i] + xp, xs + (wave + 4 * i) * 1024);
+            hv_glds16_s(wbase + (long)kb * 128, wofs[i] + wp, xs + XB + (wave + 4 * i) * 1024);
+        }
+        hv_glds4_s(sbase + (long)kb * p.x_scale_k, sofs, sXs[st]);
+        hv_glds4_s(wsp + (long)kb * p.w_scale_k, 0u, sWs[st]);
+    };
+    f32x4 acc[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int kb = k_begin; kb < min(k_begin + S - 1, k_end); ++kb) issue(kb);
+    for (int kb = k_begin; kb < k_end; ++kb) {
+        if (kb + 2 < k_end) hv_vm_wait<12>();  // two younger blocks may be in flight
+        else if (kb + 1 < k_end) hv_vm_wait<6>();
+        else hv_vm_wait<0>();
+        hv_barrier_raw();  // block kb has landed, and nobody reads block kb - 1 any more
+        if (kb + S - 1 < k_end) issue(kb + S - 1);
+        unsigned char* const xs = smem + (kb & (S - 1)) * STAGE;
+        const int left = p.K - kb * 128;
+        if (left < 128) {
+            for (int i = tid; i < 64 * 8; i += 256) {
+                const int row = i >> 3;
+                if ((i & 7) * 16 >= left) hv_st16(xs + row * 128 + (((i & 7) ^ ((row >> 1) & 7)) << 4), u32x4{0u, 0u, 0u, 0u});
+            }
+            hv_barrier_raw();
+        }
+        const unsigned char* const xrow = xs + (wave * 16 + col) * 128;
+        const unsigned char* const wrow = xs + XB + ((col >> 2) * 8 + (col & 3)) * 128;
+        const int xk = (g ^ (col >> 1)) << 4, wk = (g ^ (((col >> 1) & 1) | ((col >> 2) << 1))) << 4;
+        HvFp8Frag<WIDE> wf[4], xf;
+        xf.set(hv_ld16(xrow + xk), hv_ld16(xrow + (xk ^ 64)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) wf[i].set(hv_ld16(wrow + (i / 2) * 4096 + (i & 1) * 512 + wk), hv_ld16(wrow + (i / 2) * 4096 + (i & 1) * 512 + (wk ^ 64)));
+        const float f = sXs[kb & (S - 1)][wave * 16 + col] * sWs[kb & (S - 1)][0];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 part = hv_fp8_block_product(wf[i], xf);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][r] = fmaf(part[r], f, acc[i][r]);
+        }
+    }
+    const int m = m0 + wave * 16 + col;
+    if (m >= p.M) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int n = n0 + h * 32 + g * 8;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = acc[2 * h + i / 4][i % 4];
+        if (a.splits > 1) {
+            float* dst = p.workspace + ((long)split * p.M + m) * p.N + n;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (n + i < p.N) dst[i] = v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += p.bias && n + i < p.N ? p.bias[n + i] : 0.f;
+            hv_gemm_fp8_store(a, m, n, v);
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void hv_gemm_fp8_join_kernel(HvGemmFp8Args a) {
+    const hv_gemm_fp8_params& p = a.p;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x, all = (long)p.M * p.N;
+    if (i >= all) return;
+    const int m = (int)(i / p.N), n = (int)(i - (long)m * p.N);
+    float v = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) v += p.workspace[(long)s * all + i];
+    if (p.bias) v += p.bias[n];
+    if (p.residual) v += hv_bf2f(p.residual[(long)m * p.ldr + n]);
+    if (p.out_f32) ((float*)p.Y)[(long)m * p.ldy + n] = v;
+    else ((bf16_t*)p.Y)[(long)m * p.ldy + n] = hv_f2bf(v);
+}
+
 // ---- few rows (M <= 16 MT): the weights' bytes are what counts.  A workgroup takes 16 columns; its eight waves take the blocks
-// of the reduction in turn, operands straight from memory into registers, and their sums are joined in LDS.
+// of the reduction in turn, operands straight from memory into registers a block ahead, and their sums are joined in LDS.
 template <int MT, bool WIDE>
 __global__ __launch_bounds__(512) void hv_gemm_fp8_rows_kernel(HvGemmFp8Args a) {
     __shared__ __attribute__((aligned(16))) float red[8][MT][64][4];
@@ -323,20 +439,40 @@ __global__ __launch_bounds__(512) void hv_gemm_fp8_rows_kernel(HvGemmFp8Args a) 
         xsp[j] = p.x_scale + (long)m * p.x_scale_row;
         acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int kb = wave; kb < a.kb; kb += 8) {
+    struct Block {
+        u32x4 w[2], x[MT][2];
+        float f[MT];
+    };
+    auto load = [&](int kb) {  // what lies behind K is a repeated piece of W times zero
+        Block b;
         const int k = kb * 128 + g * 32, k1 = min(k, p.K - 16), k2 = min(k + 16, p.K - 16);
         const u32x4 zero4 = {0u, 0u, 0u, 0u};
-        HvFp8Frag<WIDE> wf;
-        wf.set(hv_ld16(wp + k1), hv_ld16(wp + k2));
+        b.w[0] = hv_ld16(wp + k1);
+        b.w[1] = hv_ld16(wp + k2);
         const float wsc = wsp[(long)kb * p.w_scale_k];
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-            HvFp8Frag<WIDE> xf;
-            xf.set(k < p.K ? hv_ld16(xp[j] + k1) : zero4, k + 16 < p.K ? hv_ld16(xp[j] + k2) : zero4);
-            const float f = xsp[j][(long)kb * p.x_scale_k] * wsc;
-            const f32x4 part = hv_fp8_block_product(wf, xf);
+            b.x[j][0] = k < p.K ? hv_ld16(xp[j] + k1) : zero4;
+            b.x[j][1] = k + 16 < p.K ? hv_ld16(xp[j] + k2) : zero4;
+            b.f[j] = xsp[j][(long)kb * p.x_scale_k] * wsc;
+        }
+        return b;
+    };
+    if (wave < a.kb) {
+        Block next = load(wave);
+        for (int kb = wave; kb < a.kb; kb += 8) {
+            const Block b = next;
+            if (kb + 8 < a.kb) next = load(kb + 8);
+            HvFp8Frag<WIDE> wf;
+            wf.set(b.w[0], b.w[1]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(part[r], f, acc[j][r]);
+            for (int j = 0; j < MT; ++j) {
+                HvFp8Frag<WIDE> xf;
+                xf.set(b.x[j][0], b.x[j][1]);
+                const f32x4 part = hv_fp8_block_product(wf, xf);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(part[r], b.f[j], acc[j][r]);
+            }
         }
     }
 #pragma unroll
@@ -356,61 +492,82 @@ __global__ __launch_bounds__(512) void hv_gemm_fp8_rows_kernel(HvGemmFp8Args a) 
     }
 }
 
-static inline long hv_gemm_fp8_workspace_of(const hv_gemm_fp8_params& p) {
+static int g_hv_gemm_fp8_tile = 0;  // hv_set_tuning(HV_TUNE_GEMM_FP8)
+
+// sizes -> kernel (its tile; 16: the rows kernel), tiles, ranges of the reduction; -1 invalid
+static inline int hv_gemm_fp8_plan(const hv_gemm_fp8_params& p, HvGemmFp8Args& a, int& tile) {
     if (p.M < 0 || p.N < 0 || p.K < 16 || p.K % 16 != 0) return -1;
+    a.p = p;
+    a.kb = (p.K + 127) / 128;
+    a.splits = 1;
+    a.per = a.kb;
+    a.tiles_m = a.tiles_n = 0;
+    auto tiles = [&](int t) { return (long)((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
+    if (tiles(64) > 0x3fffffffL) return -1;
+    const int want = g_hv_gemm_fp8_tile;
+    // 256 tiles take 3.5 times a 128 tile's CU time and run one to a CU in whole rounds, 128 tiles two to a CU (K = 2560, 36864 x 640: 95 against
+    // 78 us; 4096 x 4096 x 4096: 72 against 81); below 128 of the latter the 64 tiles' deeper pipeline and ranges are faster
+    // (1024 x 1280 x 5120: 28 against 38 us, 2048 x 1280 x 1280: 17.6 against 14.2).  An fp32 output's operands leave no room for 256.
+    const long t256 = tiles(256), t128 = tiles(128);
+    const bool large = !p.out_f32 && (t256 + 255) / 256 * 7 < 2 * (t128 < 512 ? 2 : (t128 + 255) / 256);
+    tile = p.M <= 64 ? 16 : want ? (want == 256 && p.out_f32 ? 128 : want) : large ? 256 : t128 >= 128 ? 128 : 64;
+    if (tile == 16) {
+        a.tiles_m = 1;
+        a.tiles_n = (p.N + 15) / 16;
+        return 0;
+    }
+    a.tiles_m = (p.M + tile - 1) / tile;
+    a.tiles_n = (p.N + tile - 1) / tile;
+    if (tile == 64 && a.kb >= 16 && tiles(64) > 0 && tiles(64) <= 256) {  // ranges of at least 4 blocks: a join costs what 4 - 8 blocks do
+        const long fill = 512 / tiles(64), most = a.kb / 4;
+        a.splits = (int)(fill < most ? fill : most);
+        a.per = (a.kb + a.splits - 1) / a.splits;
+        a.splits = (a.kb + a.per - 1) / a.per;
+    }
     return 0;
 }
 
-static int g_hv_gemm_fp8_tile = 0;  // hv_set_tuning(HV_TUNE_GEMM_FP8)
+static inline long hv_gemm_fp8_workspace_of(const hv_gemm_fp8_params& p) {
+    HvGemmFp8Args a;
+    int tile;
+    if (hv_gemm_fp8_plan(p, a, tile) != 0) return -1;
+    return a.splits > 1 ? (long)a.splits * p.M * p.N : 0;
+}
 
 static inline int hv_gemm_fp8_launch(const hv_gemm_fp8_params& p, hipStream_t stream) {
-    if (p.M < 0 || p.N < 0 || p.K < 16 || p.K % 16 != 0 || p.ldx % 16 != 0 || p.ldw % 16 != 0) return -1;
-    if ((((uint64_t)p.X | (uint64_t)p.W) & 15) != 0) return -1;
+    HvGemmFp8Args a;
+    int tile;
+    if (hv_gemm_fp8_plan(p, a, tile) != 0) return -1;
+    if (p.ldx % 16 != 0 || p.ldw % 16 != 0 || (((uint64_t)p.X | (uint64_t)p.W) & 15) != 0) return -1;
     if (p.ldx < 0 || p.ldw < 0 || p.ldx > (1L << 23) || p.ldw > (1L << 23)) return -1;  // 256 rows within 32-bit offsets
     if (p.x_scale_row < 0 || p.x_scale_row > (1L << 21)) return -1;
     if (p.M == 0 || p.N == 0) return 0;
-    HvGemmFp8Args a;
-    a.p = p;
-    a.kb = (p.K + 127) / 128;
+    const long floats = a.splits > 1 ? (long)a.splits * p.M * p.N : 0;
+    if (floats > p.workspace_floats || (floats > 0 && (p.workspace == nullptr || ((uint64_t)p.workspace & 3) != 0))) return -3;
     const int esz = p.out_f32 ? 4 : 2;
     a.vec = ((uint64_t)p.Y & 15) == 0 && (p.ldy * esz) % 16 == 0 && (!p.residual || (((uint64_t)p.residual & 15) == 0 && p.ldr % 8 == 0));
-    if (p.M <= 64) {
-        a.tiles_m = 1;
-        a.tiles_n = (p.N + 15) / 16;
-        hv_note("hv_gemm_fp8_rows_kernel | M=%d N=%d K=%d", p.M, p.N, p.K);
-        const dim3 grid((unsigned)a.tiles_n), block(512);
-        auto go = [&](auto wide) {
-            constexpr bool WIDE = decltype(wide)::value;
+    const long total = (long)a.tiles_m * a.tiles_n, turns = (total + 7) / 8 * 8;
+    hv_note("hv_gemm_fp8_kernel %d | M=%d N=%d K=%d ranges=%d", tile, p.M, p.N, p.K, a.splits);
+    auto go = [&](auto wide) {
+        constexpr bool WIDE = decltype(wide)::value;
+        if (tile == 16) {
+            const dim3 grid((unsigned)a.tiles_n), block(512);
             if (p.M <= 16) hv_launch(hv_gemm_fp8_rows_kernel<1, WIDE>, grid, block, stream, a);
             else if (p.M <= 32) hv_launch(hv_gemm_fp8_rows_kernel<2, WIDE>, grid, block, stream, a);
             else hv_launch(hv_gemm_fp8_rows_kernel<4, WIDE>, grid, block, stream, a);
-        };
-        if (p.out_f32) go(std::true_type{});
-        else go(std::false_type{});
-        return 0;
-    }
-    auto tiles = [&](int bm, int bn) { return (long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
-    auto set = [&](int bm, int bn, long fit) {  // fit: workgroups the chip holds at once
-        a.tiles_m = (p.M + bm - 1) / bm;
-        a.tiles_n = (p.N + bn - 1) / bn;
-        const long n = (tiles(bm, bn) + 7) / 8 * 8;
-        return dim3((unsigned)(n < fit ? n : fit));
+        } else if (tile == 256) {
+            hv_launch(hv_gemm_fp8_kernel<2, 4, 8, false>, dim3((unsigned)(turns < 256 ? turns : 256)), dim3(512), stream, a);
+        } else if (tile == 128) {
+            hv_launch(hv_gemm_fp8_kernel<2, 2, 4, WIDE>, dim3((unsigned)(turns < 512 ? turns : 512)), dim3(256), stream, a);
+        } else {
+            hv_launch(hv_gemm_fp8_small_kernel<WIDE>, dim3((unsigned)(total * a.splits)), dim3(256), stream, a);
+        }
     };
-    if (tiles(64, 64) > 0x3fffffffL) return -1;
-    if (!p.out_f32 && (g_hv_gemm_fp8_tile == 256 || (g_hv_gemm_fp8_tile == 0 && tiles(256, 256) >= 256))) {
-        const dim3 grid = set(256, 256, 256);
-        hv_note("hv_gemm_fp8_kernel<2,4,8> | M=%d N=%d K=%d", p.M, p.N, p.K);
-        hv_launch(hv_gemm_fp8_kernel<2, 4, 8, false>, grid, dim3(512), stream, a);
-    } else if (g_hv_gemm_fp8_tile >= 128 || (g_hv_gemm_fp8_tile == 0 && tiles(128, 128) >= 256)) {
-        const dim3 grid = set(128, 128, 512);
-        hv_note("hv_gemm_fp8_kernel<2,2,4> | M=%d N=%d K=%d", p.M, p.N, p.K);
-        if (p.out_f32) hv_launch(hv_gemm_fp8_kernel<2, 2, 4, true>, grid, dim3(256), stream, a);
-        else hv_launch(hv_gemm_fp8_kernel<2, 2, 4, false>, grid, dim3(256), stream, a);
-    } else {
-        const dim3 grid = set(64, 64, 1024);
-        hv_note("hv_gemm_fp8_kernel<4,1,1> | M=%d N=%d K=%d", p.M, p.N, p.K);
-        if (p.out_f32) hv_launch(hv_gemm_fp8_kernel<4, 1, 1, true>, grid, dim3(256), stream, a);
-        else hv_launch(hv_gemm_fp8_kernel<4, 1, 1, false>, grid, dim3(256), stream, a);
+    if (p.out_f32) go(std::true_type{});
+    else go(std::false_type{});
+    if (a.splits > 1) {
+        hv_note("hv_gemm_fp8_join_kernel | M=%d N=%d ranges=%d", p.M, p.N, a.splits);
+        hv_launch(hv_gemm_fp8_join_kernel, dim3((unsigned)(((long)p.M * p.N + 255) / 256)), dim3(256), stream, a);
     }
     return 0;
 }

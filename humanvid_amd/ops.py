@@ -161,14 +161,14 @@ def attention_fp8(lib, stream, q, k, vt, o, kscale, vamax, *, n_images, heads, D
     lib.call("hv_attention_fp8", C.byref(p), _p(kscale), _p(vamax), _p(kscale2), _p(vamax2), stream)
 
 
-def _on_current_device(what, *tensors):
+def _on_current_device(what, first, *others):
     """the launch goes to the current device: every tensor has to be there"""
-    dev = tensors[0].device
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
-        raise ValueError(f"{what}: tensors on {dev}, the current device is {torch.cuda.current_device()}")
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+    if dev >= 0 and dev != torch.cuda.current_device():
+        raise ValueError(f"{what}: tensors on {first.device}, the current device is {torch.cuda.current_device()}")
 
 
 def cross_attention(lib, stream, q, k, v, o, *, heads, kv_heads=None, kv_len=None, key_mask=None, scale=None, workspace=None,

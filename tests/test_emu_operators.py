@@ -132,6 +132,9 @@ def test_fp8_quantize_infinity(cx):
     (100, 133, 272, dict(layout="wide", residual=True, out=F32)),
     (70, 64, 128, dict(layout="inplace")),
     (130, 65, 16, dict(layout="odd")),
+    (70, 50, 2064, dict(residual=True)),                     # the reduction in ranges, joined
+    (66, 40, 2048, dict(layout="wide", out=F32, residual=True)),
+    (65, 70, 2560, dict(layout="inplace")),
 ])
 def test_gemm_fp8(cx, M, N, K, kw):
     oc.case_gemm_fp8(cx, M, N, K, seed=M + N + K, **kw)
@@ -145,6 +148,18 @@ def test_gemm_fp8_tiles(cx, tile):
         oc.case_gemm_fp8(cx, 65, 330, 144, seed=tile + 1, layout="wide", residual=True, out=F32)
     finally:
         cx.lib.call("hv_set_tuning", 16, 0)
+
+
+def test_gemm_fp8_ranges_need_their_workspace(cx):
+    z = torch.zeros
+    x, w = z(70, 2048, dtype=FP8), z(50, 2048, dtype=FP8)
+    a = (cx.lib, cx.stream, x, z(70, 16), w, z(1, 16), z(70, 50))
+    n = ops.gemm_fp8(*a, query_workspace=True)
+    assert n > 0
+    for bad in (None, z(n - 1)):
+        with pytest.raises(ValueError):
+            ops.gemm_fp8(*a, workspace=bad)
+    ops.gemm_fp8(*a, workspace=z(n))
 
 
 def test_operators_together(cx):

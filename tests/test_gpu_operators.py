@@ -83,6 +83,10 @@ def test_fp8_quantize(cx, M, K, rows, kw):
     (4099, 2050, 1296, dict(layout="odd")),
     (9216, 4096, 640, {}),
     (20000, 960, 320, dict(residual=True)),
+    (100, 200, 5120, dict(residual=True)),
+    (700, 333, 4112, dict(layout="wide", out=F32, residual=True)),
+    (129, 640, 2560, dict(layout="inplace")),
+    (300, 70, 5104, dict(layout="odd")),
 ])
 def test_gemm_fp8(cx, M, N, K, kw):
     oc.case_gemm_fp8(cx, M, N, K, seed=M + N + K, ref_device="cuda", **kw)
