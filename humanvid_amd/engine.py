@@ -21,6 +21,9 @@ its epilogue -- hv_groupnorm_from_parts / hv_layernorm_from_parts read kilobytes
 
 The 1-key CLIP cross-attention is algebraically a per-batch constant (softmax over one key == 1):
 to_out(to_v(e)) + bias, computed once per clip and added in the attn1 out-projection epilogue.
+Encoder states of more than one token (a text prompt, image patch tokens) are projected to keys | values once per clip and
+attended to by every spatial transformer: ln-merge, GEMM q(LN folded), hv_cross_attention, GEMM out(+residual)
+between the attn1 out-projection and the feed-forward (attention.py:410-424).
 With a FrameShard (runner.py) the images are sharded along the frame axis; around every temporal
 attention q | k | v are re-sharded frames <-> pixels by an all-to-all over RCCL (default), or the K/V
 of all frames are all-gathered (HUMANVID_TEMPORAL_EXCHANGE=allgather) -- DESIGN.md section 5.
@@ -61,6 +64,8 @@ class UNet3DEngine:
         self.bank_kv: Dict[str, tuple] = {}
         self.bank_version = None
         self.cross_const: Dict[str, torch.Tensor] = {}
+        self.cross_kv: Dict[str, torch.Tensor] = {}  # encoder states of several tokens: [batch entries][tokens][keys | values] per transformer
+        self.cross_mask: Optional[torch.Tensor] = None  # [batch entries][tokens] uint8 or None: every token
         self.do_cfg = True
         # spatial attention on the fp8 (e4m3) MFMA -- hv_attention_fp8 (transposed-V kernel family)
         # (denoising UNet only: the ReferenceNet write pass runs once per clip and keeps its banks at bf16 precision)
@@ -210,13 +215,23 @@ class UNet3DEngine:
                               for j in range(len(s.resnets) - 1 if s.kind == "mid" else len(s.resnets))]
 
     # ------------------------------------------------------------------------------------------
-    def set_encoder_hidden_states(self, ehs: torch.Tensor):
-        """ehs [B, 1, 768]: fold the one-key cross-attention of every transformer into a per-batch
-        constant (attention.py:410-424 -> to_out(to_v(e)) + bias)."""
-        assert ehs.ndim == 3 and ehs.shape[1] == 1, "the CamAnimate path feeds exactly one CLIP token"
+    def set_encoder_hidden_states(self, ehs: torch.Tensor, mask: Optional[torch.Tensor] = None):
+        """ehs [B, L, 768], one row of states per batch entry.  L == 1 without a mask: fold the one-key cross-attention of every
+        transformer into a per-batch constant (attention.py:410-424 -> to_out(to_v(e)) + bias).  Otherwise: project the states to
+        keys | values; the transformers attend to them, to the tokens only where mask [B, L] is non-zero (an entry without any token
+        gets to_out's bias)."""
+        if ehs.ndim != 3 or ehs.shape[1] < 1:
+            raise ValueError(f"encoder_hidden_states: [batch, tokens, channels] with at least one token expected, got {tuple(ehs.shape)}")
+        if mask is not None and tuple(mask.shape) != tuple(ehs.shape[:2]):
+            raise ValueError(f"encoder_attention_mask: {tuple(ehs.shape[:2])} expected, got {tuple(mask.shape)}")
         B = ehs.shape[0]
-        e = self._dev(ehs[:, 0], BF16)
         st = self.stream
+        if ehs.shape[1] > 1 or mask is not None:
+            self._set_cross_states(ehs, mask)
+            return
+        self.cross_kv.clear()
+        self.cross_mask = None
+        e = self._dev(ehs[:, 0], BF16)
         for loc in self.locations:
             t = loc + ".transformer_blocks.0"
             C = self.w[t + ".attn2.to_out.0.w"].shape[0]
@@ -227,6 +242,57 @@ class UNet3DEngine:
                 c = torch.empty(B, C, dtype=F32, device=self.device)
                 self.cross_const[loc] = c
             ops.gemm(self.lib, st, v, self.w[t + ".attn2.to_out.0.w"], c, bias=self.w[t + ".attn2.to_out.0.bias"])
+
+    def _set_cross_states(self, ehs: torch.Tensor, mask: Optional[torch.Tensor]):
+        B, tokens, _ = ehs.shape
+        if self.locations and (self.locations[0] + ".transformer_blocks.0.attn2.q.w") not in self.w:  # first use: their weights
+            sd = self.unet.state_dict()
+            for loc in self.locations:
+                t = loc + ".transformer_blocks.0"
+                gamma, beta = sd[t + ".norm2.weight"].float(), sd[t + ".norm2.bias"].float()
+                wf, colsum, bf = packing.fold_layernorm(sd[t + ".attn2.to_q.weight"].float(), None, gamma, beta)
+                self.w[t + ".attn2.q.w"] = self._dev(wf)
+                self.w[t + ".attn2.q.colsum"], self.w[t + ".attn2.q.bias"] = self._dev(colsum, F32), self._dev(bf, F32)
+                self.w[t + ".attn2.kv.w"] = self._dev(packing.pack_linear(torch.cat(
+                    [sd[t + ".attn2.to_k.weight"], sd[t + ".attn2.to_v.weight"]], dim=0).float()))
+        x = self._dev(ehs.reshape(B * tokens, -1), BF16)
+        old = dict(self.cross_kv)
+        self.cross_kv.clear()  # (in place: executors of one half share the table)
+        for loc in self.locations:
+            w = self.w[loc + ".transformer_blocks.0.attn2.kv.w"]
+            kv = old.get(loc)
+            if kv is None or kv.shape != (B, tokens, w.shape[0]):  # (the same buffers again where they fit: a recorded step reads them)
+                kv = torch.empty(B, tokens, w.shape[0], dtype=BF16, device=self.device)
+            ops.gemm(self.lib, self.stream, x, w, kv.view(B * tokens, -1))
+            self.cross_kv[loc] = kv
+        if mask is None:
+            self.cross_mask = None
+        else:
+            m = (mask != 0).to(device=self.device, dtype=torch.uint8)
+            if self.cross_mask is not None and self.cross_mask.shape == m.shape:
+                self.cross_mask.copy_(m)
+            else:
+                self.cross_mask = m.contiguous()
+
+    def _cross_attention(self, loc: str, hid: torch.Tensor, B: int):
+        """hid [(B rows), C] += to_out(attention(norm2(hid), encoder states)) + bias (attention.py:410-424)"""
+        L, st, w, ws = self.lib, self.stream, self.w, self.ws
+        t = loc + ".transformer_blocks.0"
+        M, C = hid.shape
+        kv, mask = self.cross_kv[loc], self.cross_mask
+        if self.cfg_half is not None and B == 1:
+            kv = kv[self.cfg_half:self.cfg_half + 1]
+            mask = None if mask is None else mask[self.cfg_half:self.cfg_half + 1]
+        if kv.shape[0] != B:
+            raise ValueError(f"encoder_hidden_states: {kv.shape[0]} batch entries for a batch of {B}")
+        mean, rstd = self.run.ln_stats(hid)
+        q, o = ws.get(f"tr_xq_{M}x{C}", (M, C)), ws.get(f"tr_o_{M}x{C}", (M, C))
+        ops.gemm(L, st, hid, w[t + ".attn2.q.w"], q, bias=w[t + ".attn2.q.bias"], row_mean=mean, row_rstd=rstd,
+                 colsum=w[t + ".attn2.q.colsum"])
+        qb, ob, kw = q.view(B, M // B, C), o.view(B, M // B, C), dict(heads=self.heads, key_mask=mask)
+        n = ops.cross_attention(L, st, qb, kv[..., :C], kv[..., C:], ob, query_workspace=True, **kw)
+        ops.cross_attention(L, st, qb, kv[..., :C], kv[..., C:], ob, workspace=ws.get("tr_xws", (n,), F32) if n else None, **kw)
+        self.run.gemm_ln(o, w[t + ".attn2.to_out.0.w"], hid, bias=w[t + ".attn2.to_out.0.bias"], residual=hid)
 
     def set_reference_banks(self, banks: Optional[Dict[str, torch.Tensor]], do_cfg: bool):
         """banks: {transformer location -> [b, Nb, C]} (norm1 features of the ReferenceNet write pass,
@@ -277,7 +343,7 @@ class UNet3DEngine:
         self.set_reference_banks(banks, do_cfg=bool(mode.get("do_cfg")))
 
     # ------------------------------------------------------------------------------------------
-    def forward_ncfhw(self, sample, timestep, encoder_hidden_states, pose_cond_fea):
+    def forward_ncfhw(self, sample, timestep, encoder_hidden_states, pose_cond_fea, encoder_attention_mask=None):
         """The reference's tensor interface: sample [b,c,f,h,w] -> [b,c_out,f,h,w] (same dtype)."""
         if sample.device.type != "cuda":
             raise RuntimeError("UNet3DConditionModel.forward needs CUDA/HIP tensors: there is no CPU path")
@@ -288,7 +354,7 @@ class UNet3DEngine:
         self._banks_from_modules()
         # the folded cross-attention constants are recomputed on every call of the tensor interface (32 tiny GEMMs): a
         # cache keyed on the embedding's address would go stale when the allocator reuses the address for the next clip
-        self.set_encoder_hidden_states(encoder_hidden_states)
+        self.set_encoder_hidden_states(encoder_hidden_states, encoder_attention_mask)
         st = self.stream
         src = sample if sample.dtype in (F32, BF16) else sample.float()
         x_in = self.ws.get("x_in", (b * f, h, w, packing.round_up(c, 32)))
@@ -305,13 +371,13 @@ class UNet3DEngine:
         ops.unpack_nhwc(self.lib, st, y, out)
         return out.to(sample.dtype)
 
-    def forward_reference(self, sample, timestep, encoder_hidden_states):
+    def forward_reference(self, sample, timestep, encoder_hidden_states, encoder_attention_mask=None):
         """ReferenceNet pass: sample [b,4,h,w] -> last hidden state [b,C0,h,w]; fills `bank` of every
         BasicTransformerBlock when the model is in write mode (pipeline_pose2vid_long.py:470-480)."""
         if sample.device.type != "cuda":
             raise RuntimeError("UNet2DConditionModel.forward needs CUDA/HIP tensors: there is no CPU path")
         b, c, h, w_ = sample.shape
-        self.set_encoder_hidden_states(encoder_hidden_states)  # every call: see forward_ncfhw
+        self.set_encoder_hidden_states(encoder_hidden_states, encoder_attention_mask)  # every call: see forward_ncfhw
         self.bank_kv = {}
         st = self.stream
         src = sample if sample.dtype in (F32, BF16) else sample.float()
@@ -463,11 +529,19 @@ class UNet3DEngine:
             else:
                 ops.attention(L, st, qk, qk[:, C:], vt, o, n_images=n, heads=self.heads, D=C // self.heads, Lq=N, L1=N,
                               ldq=ldqk, ldk=ldqk, ldvt=ldvt, ldo=C, **kw)
+            if self.cross_kv:
+                self.run.gemm_ln(o, w[t + ".attn1.to_out.0.w"], hid, bias=w[t + ".attn1.to_out.0.bias"], residual=hid)
+                self._cross_attention(prefix, hid, B)
+                return finish(prefix, x, hid, N, x2d)
             cc = self.cross_const[prefix]  # [batch entries][C]: the folded 1-key cross-attention, one row per CFG half
             if self.cfg_half is not None and B == 1:
                 cc = cc[self.cfg_half:self.cfg_half + 1]
             self.run.gemm_ln(o, w[t + ".attn1.to_out.0.w"], hid, bias=w[t + ".attn1.to_out.0.bias"],
                              rowvec=cc, rowvec_period=F * N, residual=hid)
+            return finish(prefix, x, hid, N, x2d)
+
+        def finish(prefix, x, hid, N, x2d):
+            t = prefix + ".transformer_blocks.0"
             feed_forward(t + ".ff1", t + ".ff.net.2", hid)
             self.run.gemm_with_stats(hid, w[prefix + ".proj_out.w"], x, N, bias=w[prefix + ".proj_out.bias"], residual=x2d)
             return x

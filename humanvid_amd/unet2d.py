@@ -163,8 +163,9 @@ class UNet2DConditionModel(nn.Module):
         return self._engine
 
     @torch.no_grad()
-    def forward(self, sample, timestep, encoder_hidden_states, return_dict: bool = True, **unused):
-        """sample [b,4,h,w].  In write mode (ReferenceAttentionControl) fills the banks; returns the
+    def forward(self, sample, timestep, encoder_hidden_states, return_dict: bool = True, encoder_attention_mask=None, **unused):
+        """sample [b,4,h,w], encoder_hidden_states [b, tokens, channels] (one token or several), encoder_attention_mask [b, tokens]:
+        the tokens that are attended to (non-zero).  In write mode (ReferenceAttentionControl) fills the banks; returns the
         last up-block's hidden state like the reference (its conv_out is commented out)."""
-        out = self.engine().forward_reference(sample, timestep, encoder_hidden_states)
+        out = self.engine().forward_reference(sample, timestep, encoder_hidden_states, encoder_attention_mask)
         return (out,) if not return_dict else FrozenConfig(sample=out)

@@ -413,11 +413,13 @@ class UNet3DConditionModel(nn.Module):
     @torch.no_grad()
     def forward(self, sample, timestep, encoder_hidden_states, class_labels=None, pose_cond_fea=None,
                 attention_mask=None, down_block_additional_residuals=None, mid_block_additional_residual=None,
-                return_dict: bool = True) -> Union[UNet3DConditionOutput, Tuple]:
+                return_dict: bool = True, encoder_attention_mask=None) -> Union[UNet3DConditionOutput, Tuple]:
+        """encoder_hidden_states [b, tokens, channels]: one token (the CLIP image embedding) or several; encoder_attention_mask
+        [b, tokens]: the tokens that are attended to (non-zero), all by default."""
         if attention_mask is not None or down_block_additional_residuals is not None or \
                 mid_block_additional_residual is not None or class_labels is not None:
             raise NotImplementedError("attention_mask / additional residuals / class_labels are unused on this path")
-        out = self.engine().forward_ncfhw(sample, timestep, encoder_hidden_states, pose_cond_fea)
+        out = self.engine().forward_ncfhw(sample, timestep, encoder_hidden_states, pose_cond_fea, encoder_attention_mask)
         if not return_dict:
             return (out,)
         return UNet3DConditionOutput(sample=out)
