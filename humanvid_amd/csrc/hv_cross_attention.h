@@ -830,12 +830,12 @@ static inline int hv_cross_attention_launch(const hv_cross_attention_params& p, 
     HvCrossArgs a;
     const int rc = hv_cross_attention_plan(p, a);
     if (rc) return rc;
-    if (!(p.scale > 0.f) || p.scale > 3.0e38f) return -1;
+    if (!(p.scale > 0.f) || p.scale > 1.0e30f) return -1;
     if (p.B == 0 || p.Lq == 0) return 0;
-    if (p.ldk < 0 || p.ldv < 0 || p.ldk > (1L << 24) || p.ldv > (1L << 24)) return -1;  // 64 rows within 32-bit offsets
     const uint64_t addr = (uint64_t)p.Q | (uint64_t)p.K | (uint64_t)p.V | (uint64_t)p.O;
     const long strides = p.ldq | p.ldk | p.ldv | p.ldo | p.q_stride_b | p.k_stride_b | p.v_stride_b | p.o_stride_b;
-    if ((addr & 15) != 0 || (strides & 7) != 0) return -1;
+    if ((addr & 15) != 0 || (strides & 7) != 0 || (strides | p.mask_stride_b) < 0) return -1;
+    if (p.ldk > (1L << 24) || p.ldv > (1L << 24)) return -1;  // 64 rows within 32-bit offsets
     if (hv_cross_attention_floats(a) > p.workspace_floats || (a.splits > 1 && (p.workspace == nullptr || ((uint64_t)p.workspace & 15) != 0))) return -3;
     switch (p.D) {
         case 40: hv_cross_attention_launch_d<40>(a, stream); break;

@@ -496,7 +496,7 @@ static int g_hv_gemm_fp8_tile = 0;  // hv_set_tuning(HV_TUNE_GEMM_FP8)
 
 // sizes -> kernel (its tile; 16: the rows kernel), tiles, ranges of the reduction; -1 invalid
 static inline int hv_gemm_fp8_plan(const hv_gemm_fp8_params& p, HvGemmFp8Args& a, int& tile) {
-    if (p.M < 0 || p.N < 0 || p.K < 16 || p.K % 16 != 0) return -1;
+    if (p.M < 0 || p.N < 0 || p.K < 16 || p.K % 16 != 0 || p.M > 0x7fffff00 || p.N > 0x7fffff00 || p.K > 0x7fffff00) return -1;
     a.p = p;
     a.kb = (p.K + 127) / 128;
     a.splits = 1;
@@ -540,7 +540,7 @@ static inline int hv_gemm_fp8_launch(const hv_gemm_fp8_params& p, hipStream_t st
     if (hv_gemm_fp8_plan(p, a, tile) != 0) return -1;
     if (p.ldx % 16 != 0 || p.ldw % 16 != 0 || (((uint64_t)p.X | (uint64_t)p.W) & 15) != 0) return -1;
     if (p.ldx < 0 || p.ldw < 0 || p.ldx > (1L << 23) || p.ldw > (1L << 23)) return -1;  // 256 rows within 32-bit offsets
-    if (p.x_scale_row < 0 || p.x_scale_row > (1L << 21)) return -1;
+    if (p.x_scale_row < 0 || p.x_scale_row > (1L << 21) || (p.M > 1 && p.ldy < p.N) || p.ldr < 0) return -1;
     if (p.M == 0 || p.N == 0) return 0;
     const long floats = a.splits > 1 ? (long)a.splits * p.M * p.N : 0;
     if (floats > p.workspace_floats || (floats > 0 && (p.workspace == nullptr || ((uint64_t)p.workspace & 3) != 0))) return -3;
@@ -680,7 +680,8 @@ __global__ __launch_bounds__(256) void hv_fp8_quantize_blocks_kernel(HvQuantArgs
 
 static inline int hv_fp8_quantize_launch(const HvQuantArgs& in, int block_rows, hipStream_t stream) {
     HvQuantArgs a = in;
-    if (a.M < 0 || a.K <= 0 || a.K % 16 != 0 || a.ldx % 8 != 0 || a.ldq % 16 != 0 || (block_rows != 1 && block_rows != 128)) return -1;
+    if (a.M < 0 || a.K <= 0 || a.K % 16 != 0 || a.K > 0x7fffff00 || a.M > 0x7fffff00 || a.ldx % 8 != 0 || a.ldq % 16 != 0) return -1;
+    if ((block_rows != 1 && block_rows != 128) || (a.M > 1 && (a.ldq < a.K || a.ldx < 0))) return -1;
     if ((((uint64_t)a.X | (uint64_t)a.Q) & 15) != 0) return -1;
     if (a.M == 0) return 0;
     a.kb = (a.K + 127) / 128;

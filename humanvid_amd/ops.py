@@ -171,12 +171,21 @@ def _on_current_device(what, first, *others):
         raise ValueError(f"{what}: tensors on {first.device}, the current device is {torch.cuda.current_device()}")
 
 
+def _overlaps(n0, s0, n1, s1, width):
+    """do the rows of [n0, n1, width] with strides s0, s1, 1 share elements?"""
+    if n0 > 1 and n1 > 1:
+        if s0 < s1:
+            n0, s0, n1, s1 = n1, s1, n0, s0
+        return s1 < width or s0 < (n1 - 1) * s1 + width
+    return (n0 > 1 and s0 < width) or (n1 > 1 and s1 < width)
+
+
 def cross_attention(lib, stream, q, k, v, o, *, heads, kv_heads=None, kv_len=None, key_mask=None, scale=None, workspace=None,
                     query_workspace=False):
     """o[b, i] = softmax(scale q[b, i] . k[b, j]) v[b, j] per head, over the attended states j: j < kv_len[b], key_mask[b, j] != 0.
     q, o [B, Lq, heads * D], k, v [B, Lk, kv_heads * D] bf16 views (last dimension contiguous, other strides multiples of 8; k, v may be
     expanded over the batch); heads // kv_heads query heads share a key head.  kv_len int32 [B], key_mask uint8 / bool [B, Lk] on the
-    device.  An entry that attends to nothing gets zeros.  scale: 1 / sqrt(D) by default.  o may be q.
+    device.  An entry that attends to nothing gets zeros.  scale: 1 / sqrt(D) by default.  o may be q, and overlap nothing else.
     query_workspace=True launches nothing and returns the fp32 elements `workspace` needs for these sizes (0: none)."""
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or o.shape != q.shape:
         raise ValueError("cross_attention: q, o [B, Lq, heads * D] and k, v [B, Lk, kv_heads * D] expected")
@@ -191,6 +200,8 @@ def cross_attention(lib, stream, q, k, v, o, *, heads, kv_heads=None, kv_len=Non
     sq, sk, sv, so = q.stride(), k.stride(), v.stride(), o.stride()
     if Cq > 1 and (sq[2] != 1 or so[2] != 1 or sk[2] != 1 or sv[2] != 1):
         raise ValueError("cross_attention: the last dimension must be contiguous")
+    if _overlaps(B, so[0], Lq, so[1], Cq):
+        raise ValueError("cross_attention: the rows of o must not overlap")
     ms = 0
     if kv_len is not None and (kv_len.dtype != torch.int32 or kv_len.shape != (B,) or not kv_len.is_contiguous()):
         raise ValueError("cross_attention: kv_len must be contiguous int32 [B]")
@@ -229,6 +240,8 @@ def fp8_quantize(lib, stream, x, q, scale, *, block_rows=1):
         raise ValueError(f"fp8_quantize: scale {tuple(scale.shape)}, expected {(-(-M // block_rows), -(-K // 128))}")
     if (K > 1 and (x.stride(1) != 1 or q.stride(1) != 1)) or (M > 1 and q.stride(0) < K):
         raise ValueError("fp8_quantize: the rows of x and q must be contiguous, those of q must not overlap")
+    if _overlaps(scale.shape[0], scale.stride(0), scale.shape[1], scale.stride(1), 1):
+        raise ValueError("fp8_quantize: the elements of scale must not overlap")
     _on_current_device("fp8_quantize", x, q, scale)
     lib.call("hv_fp8_quantize", x.data_ptr(), x.stride(0), M, K, block_rows, q.data_ptr(), q.stride(0), scale.data_ptr(),
              scale.stride(0), scale.stride(1), stream)

@@ -222,9 +222,9 @@ int hv_attention_fp8(const hv_attention_params* p, const float* kscale, const fl
  * O[b][i][h] = sum_j softmax_j(scale Q[b][i][h] . K[b][j][g]) V[b][j][g],  g = h / (heads / kv_heads), over the attended states:
  * j < kv_len[b] and key_mask[b][j] != 0.  A batch entry with no attended state gets zeros; what memory holds in the other
  * states (NaN included) does not reach the output, and states at or behind kv_len are not read.  Values are row-major.  All frames of a
- * clip that share their half's prompt are ONE batch entry (Lq = frames * tokens).  O may be Q.  Any Lq, Lk >= 0; D in
- * {40, 64, 80, 128, 160}; pointers 16-byte aligned, strides multiples of 8 elements (the batch strides of K, V and the mask may be 0:
- * shared states).  The keys are cut into ranges that are joined by a second launch where the queries alone would not fill the
+ * clip that share their half's prompt are ONE batch entry (Lq = frames * tokens).  O may be Q, and overlap nothing else.  Any Lq, Lk >= 0; D in
+ * {40, 64, 80, 128, 160}; pointers 16-byte aligned, strides >= 0 in multiples of 8 elements (the batch strides of K, V and the mask may be 0:
+ * shared states; rows of K and V at most 2^24 elements apart).  The keys are cut into ranges that are joined by a second launch where the queries alone would not fill the
  * chip: hv_cross_attention_workspace() floats of scratch, not to be shared by calls that may run at the same time. */
 typedef struct hv_cross_attention_params {
     const uint16_t* Q; /* row i of entry b at Q + b * q_stride_b + i * ldq, head h at column h*D */
@@ -239,7 +239,7 @@ typedef struct hv_cross_attention_params {
     const uint8_t* key_mask; /* device [B][Lk] bytes, row stride mask_stride_b, or NULL */
     long mask_stride_b;
     int B, Lq, Lk, heads, kv_heads, D;
-    float scale; /* > 0, finite */
+    float scale; /* in (0, 1e30] */
     float* workspace;
     long workspace_floats;
 } hv_cross_attention_params;

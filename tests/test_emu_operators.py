@@ -214,6 +214,29 @@ def test_cross_attention_refuses_strides(cx):
         ops.cross_attention(cx.lib, cx.stream, q, k, k, torch.zeros(1, 2, 40, dtype=BF16), heads=1)
 
 
+def test_outputs_that_overlap_themselves_are_refused(cx):
+    q, k = torch.zeros(2, 3, 40, dtype=BF16), torch.zeros(2, 3, 40, dtype=BF16)
+    for o in (torch.zeros(1, 3, 40, dtype=BF16).expand(2, -1, -1), torch.zeros(2, 1, 40, dtype=BF16).expand(-1, 3, -1)):
+        with pytest.raises(ValueError):
+            ops.cross_attention(cx.lib, cx.stream, q, k, k, o, heads=1)
+    o = torch.zeros(3, 2, 40, dtype=BF16).transpose(0, 1)  # queries outside, entries inside: fine
+    ops.cross_attention(cx.lib, cx.stream, q, k, k, o, heads=1)
+    x, w = torch.zeros(4, 64, dtype=FP8), torch.zeros(8, 64, dtype=FP8)
+    with pytest.raises(ValueError):
+        ops.gemm_fp8(cx.lib, cx.stream, x, torch.zeros(4, 1), w, torch.zeros(1, 1), torch.zeros(1, 8).expand(4, -1))
+    with pytest.raises(ValueError):
+        ops.fp8_quantize(cx.lib, cx.stream, torch.zeros(4, 256, dtype=BF16), torch.zeros(4, 256, dtype=FP8), torch.zeros(1, 2).expand(4, -1))
+
+
+def test_gemm_fp8_residual_of_one_row(cx):
+    """a residual that is the same row for all (stride 0)"""
+    x, xs, w, ws, _, res = oc.gemm_operands(70, 64, 128, 3)
+    y, want = torch.empty(70, 64), torch.empty(70, 64)
+    ops.gemm_fp8(cx.lib, cx.stream, x, xs, w, ws, y, residual=res[:1].expand(70, -1))
+    ops.gemm_fp8(cx.lib, cx.stream, x, xs, w, ws, want, residual=res[:1].expand(70, -1).contiguous())
+    assert torch.equal(y, want)
+
+
 def _quant(cx, x=(4, 64), xt=BF16, q=None, qt=FP8, scale=(4, 1), st=F32, **kw):
     ops.fp8_quantize(cx.lib, cx.stream, torch.zeros(*x, dtype=xt), torch.zeros(*(q or x), dtype=qt), torch.zeros(*scale, dtype=st), **kw)
 
@@ -251,6 +274,13 @@ def test_null_operands_are_refused(cx):
     p.Lq = -1
     assert cx.lib.cdll.hv_cross_attention(C.byref(p), None) == A.HV_EINVAL
     assert cx.lib.cdll.hv_cross_attention_workspace(C.byref(p)) == A.HV_EINVAL
+    for field, value in (("ldq", -8), ("k_stride_b", -40), ("ldk", 1 << 25), ("mask_stride_b", -1)):
+        buf = torch.zeros(64, dtype=BF16)
+        p = A.CrossAttentionParams(B=1, Lq=1, Lk=1, heads=1, kv_heads=1, D=40, scale=1.0, Q=buf.data_ptr(), K=buf.data_ptr(), V=buf.data_ptr(),
+                                   O=buf.data_ptr(), ldq=40, ldk=40, ldv=40, ldo=40)
+        assert cx.lib.cdll.hv_cross_attention(C.byref(p), None) == A.HV_OK
+        setattr(p, field, value)
+        assert cx.lib.cdll.hv_cross_attention(C.byref(p), None) == A.HV_EINVAL, field
     r = A.GemmFp8Params(M=1, N=1, K=16)
     assert cx.lib.cdll.hv_gemm_fp8(C.byref(r), None) == A.HV_EINVAL
     assert cx.lib.cdll.hv_gemm_fp8(None, None) == A.HV_EINVAL
