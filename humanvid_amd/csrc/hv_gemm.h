@@ -63,8 +63,8 @@ HV_DEV int hv_swz_wperm(int row, int chunk) {  // BK = 64: 128-byte rows, 8 chun
 //   gelu(x) = x Phi(x) = max(x, 0) - |x| / 2 * erfc(|x| / sqrt 2),   erfc(|x| / sqrt 2) = 2^(u q(u)), u = min(|x|, 4 sqrt 2)
 // with q a degree-5 polynomial fitted (weighted minimax, oracle-side check in tests/kernel_cases.py case_gemm_geglu) to
 // log2 erfc on [0, 4]: |gelu error| < 6e-7 absolute, < 5e-4 of max(|gelu|, 1e-3) -- below the bf16 rounding of the output
-// (2^-9) everywhere.  One transcendental (v_exp_f32) and the polynomial in packed fp32 (v_pk_fma_f32: two elements per
-// instruction), against one rcp + one exp2 + 12 scalar VALU per element of the Abramowitz-Stegun 7.1.26 form of rounds 1-2:
+// (2^-9) everywhere.  One transcendental (v_exp_f32) and the polynomial (pairs in the source, one v_fma_f32 per element: the packed
+// fp32 instructions are off, see humanvid_amd/build.py), against one rcp + one exp2 + 12 scalar VALU per element of the Abramowitz-Stegun 7.1.26 form of rounds 1-2:
 // the GEGLU epilogue of a 256 x 256 tile was VALU-bound on it (5000 of the tile's 33 000 cycles at K = 320).
 HV_DEV f32x2 hv_gelu_times2(f32x2 x, f32x2 h) {
     const f32x2 u = {fminf(fabsf(x[0]), 5.656854249f), fminf(fabsf(x[1]), 5.656854249f)};

@@ -4,7 +4,8 @@
 //   y[m][n] = bias[n] + residual[m][n] + sum_kb xs[m][kb] ws[n / 128][kb] sum_{k in block kb} x8[m][k] w8[n][k]
 //
 // A block of 128 is exactly one v_mfma_f32_16x16x128_f8f6f4: every instruction starts from a zero accumulator and its four
-// results per lane are added to the fp32 sums with the block's factor xs ws -- 4 v_fma per 32-cycle MFMA, which fit under it.
+// results per lane are added to the fp32 sums with the block's factor xs ws -- 4 v_fma per 32-cycle MFMA, 16 cycles that the matrix pipe
+// does not hide.
 // The operands are taken as A = W (rows n), B = X (columns m): a lane then owns ONE row m of Y per 16-row tile, so xs is one
 // value per lane and tile, and the four W tiles of a 64-column block are read from LDS in an order that leaves the lane twice
 // 8 consecutive columns: 16-byte stores, the four lanes of a row 64 bytes in one.

@@ -290,7 +290,7 @@ long hv_gemm_fp8_workspace(const hv_gemm_fp8_params* p); /* floats of scratch hv
 #define HV_TUNE_CONV_RASTER 9    /* workgroup raster of hv_conv3x3 inside an XCD: 0 = the output-channel tiles of a pixel patch adjacent (halo shared through L2, weights re-streamed), 1 = the pixel patches of an output-channel tile adjacent (weights stay in L2), 2 (default) = 1 where Cin x Cout >= 640 x 640: HBM-side fetch of the 1280 -> 1280 convolution 1.4 -> 0.6 GB per launch at equal time (profiles/r04_s3.txt) */
 #define HV_TUNE_CONV_W4 12       /* stride-1 convolutions of a plain single-source input with Cout % 320 == 0 or Cout % 256 == 0 on hv_conv_w4_kernel (hv_conv4.h: 12 x 16 pixels x 320 / 256 channels on four waves, halo and weights by LDS-DMA; the width whose tiles fill the rounds of 256 CUs better): 1 (default) = where the tiles fill their rounds of 256 CUs to >= 70 % (>= 128 tiles) and the patches cover >= 80 % of the image, 0 = never, 2 = wherever the structure allows (tests), 3 = as 1 with 320-channel tiles only (A/B) */
 #define HV_TUNE_CMDLIST_GRAPHS 7 /* 1 (default): hv_cmdlist_run replays a recorded segment as ONE captured HIP graph; 0: re-issues its launches one by one (A/B) */
-#define HV_TUNE_GEMM_FP8 16      /* hv_gemm_fp8 with M > 64: 0 (default) = the largest tile that still gives every CU one; 64 / 128 / 256 = square tiles of that size (tests) */
+#define HV_TUNE_GEMM_FP8 16      /* hv_gemm_fp8 with M > 64: 0 (default) = the square tile (256, 128, 64) whose rounds over the CUs take least; 64 / 128 / 256 = that one (tests; an fp32 output takes 128 for 256) */
 int hv_set_tuning(int key, int value);
 
 /* ---- temporal self-attention over the frame axis ------------------------------------------
