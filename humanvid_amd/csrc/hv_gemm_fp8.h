@@ -135,8 +135,10 @@ HV_DEV void hv_gemm_fp8_store(const HvGemmFp8Args& a, int m, int n, float* v) {
 // results are stored -- one workgroup fills a CU's registers and LDS, so nothing else would cover that (147456 x 960 x 320: 131 -> 124 us;
 // 18432 x 10240 x 1280: 309 -> 306).
 // What bounds it: per block and wave 32 MFMAs (1024 cycles) and 128 fused multiply-adds for the block's scales (4 cycles each, which the
-// matrix pipe does not hide), twice that per SIMD, of 5800 measured: 0.77 of what the two take one after the other; short
-// reductions by the stores (283 MB of the 330 MB at K = 320).
+// matrix pipe does not hide); a 256 x 256 tile takes 2.2 - 2.5 us a block (1640 - 1690 TFLOP/s at K = 1280).  Short reductions: the stores
+// (283 MB of the 330 MB at 147456 x 960 x 320), of which a tile's first block covers its predecessor's: 20 us for a block of all tiles,
+// 50 - 60 us for the results whatever K is.  (The second block requested ahead of the stores too costs a barrier more and was slower: 138.)
+// A whole tile's residual is requested four row tiles at a time (18432 x 10240 x 1280: 407 -> 376 us, 147456 x 960 x 320: 191 -> 182).
 template <int WM, int WN, int MT, bool WIDE>
 __global__ __launch_bounds__(64 * WM * WN, 2) void hv_gemm_fp8_kernel(HvGemmFp8Args a) {
     constexpr int BM = WM * MT * 16, BN = WN * 64, WAVES = WM * WN;
@@ -204,7 +206,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void hv_gemm_fp8_kernel(HvGemmFp8A
     place(t);
     issue(0, 0);
     issue_bias(0);
-    bool stores = false;  // the last tile's 2 MT stores, and nothing else, are younger than the copies in flight
+    constexpr int SN = (WIDE ? 4 : 2) * MT;  // stores of a whole tile per lane
+    bool stores = false;  // the last tile's SN stores, and nothing else, are younger than the copies in flight
     for (int st = 0, odd = 0;; odd ^= 1) {
         const int mt = m0, nt = n0;  // this tile
         const int next = t + turn;
@@ -214,7 +217,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void hv_gemm_fp8_kernel(HvGemmFp8A
 #pragma unroll
             for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int kb = 0; kb < a.kb; ++kb, st ^= 1) {
-            if (kb == 0 && stores) hv_vm_wait<2 * MT>();
+            if (kb == 0 && stores) hv_vm_wait<SN>();
             else hv_vm_wait<0>();
             hv_barrier_raw();  // block kb has landed, and nobody reads the other stage any more
             const float wsc = wnext;
@@ -276,17 +279,47 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void hv_gemm_fp8_kernel(HvGemmFp8A
 #pragma unroll
             for (int e = 0; e < 4; ++e) bias[i + e] = b[e];
         }
-        stores = !WIDE && a.vec && p.residual == nullptr && mt + BM <= p.M && nt + BN <= p.N;
+        stores = a.vec && mt + BM <= p.M && nt + BN <= p.N;
         if (stores) {
-            bf16_t* y = (bf16_t*)p.Y + (long)(mt + wm * MT * 16 + col) * p.ldy + n;
+            const long at = (long)(mt + wm * MT * 16 + col);
+            char* y = (char*)p.Y + (at * p.ldy + n) * (WIDE ? 4 : 2);
+            auto rows = [&](auto residual) {
+                constexpr int RB = 4;  // row tiles whose residual is on its way at once
+                const bf16_t* r = residual ? p.residual + at * p.ldr + n : nullptr;
 #pragma unroll
-            for (int j = 0; j < MT; ++j, y += 16 * p.ldy) {
-                float v[16];
+                for (int jb = 0; jb < MT; jb += RB) {
+                    u32x4 res[RB][2];
+                    if (residual) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = acc[i / 4][j][i % 4] + bias[i];
-                hv_st16(y, hv_pack8(v));
-                hv_st16(y + 32, hv_pack8(v + 8));
-            }
+                        for (int j = 0; j < RB; ++j, r += 16 * p.ldr) {
+                            res[j][0] = hv_ld16(r);
+                            res[j][1] = hv_ld16(r + 32);
+                        }
+                        hv_sched_fence();
+                    }
+#pragma unroll
+                    for (int j = 0; j < RB; ++j, y += 16 * p.ldy * (WIDE ? 4 : 2)) {
+                        float v[16], f[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = acc[i / 4][jb + j][i % 4] + bias[i];
+                        if (residual) {
+                            hv_unpack8(res[j][0], f);
+                            hv_unpack8(res[j][1], f + 8);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) v[i] += f[i];
+                        }
+                        if (WIDE) {
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4) *reinterpret_cast<f32x4*>(y + (i / 8 * 32 + i % 8) * 4) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+                        } else {
+                            hv_st16((bf16_t*)y, hv_pack8(v));
+                            hv_st16((bf16_t*)y + 32, hv_pack8(v + 8));
+                        }
+                    }
+                }
+            };
+            if (p.residual) rows(std::true_type{});
+            else rows(std::false_type{});
         } else {
 #pragma unroll
             for (int j = 0; j < MT; ++j) {

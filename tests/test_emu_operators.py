@@ -145,6 +145,8 @@ def test_gemm_fp8_tiles(cx, tile):
     cx.lib.call("hv_set_tuning", 16, tile)
     try:
         oc.case_gemm_fp8(cx, 270, 200, 272, seed=tile, residual=True)
+        oc.case_gemm_fp8(cx, 260, 264, 144, seed=tile + 2, layout="inplace")
+        oc.case_gemm_fp8(cx, 140, 136, 144, seed=tile + 3, residual=True, out=F32)
         oc.case_gemm_fp8(cx, 65, 330, 144, seed=tile + 1, layout="wide", residual=True, out=F32)
     finally:
         cx.lib.call("hv_set_tuning", 16, 0)

@@ -97,6 +97,8 @@ def test_gemm_fp8_tiles(cx, tile):
     cx.lib.call("hv_set_tuning", 16, tile)
     try:
         oc.case_gemm_fp8(cx, 1541, 1000, 1040, seed=tile, residual=True, ref_device="cuda")
+        oc.case_gemm_fp8(cx, 4100, 1288, 400, seed=tile + 2, layout="inplace", ref_device="cuda")
+        oc.case_gemm_fp8(cx, 2100, 1288, 400, seed=tile + 3, residual=True, out=F32, ref_device="cuda")
         oc.case_gemm_fp8(cx, 300, 330, 144, seed=tile + 1, layout="wide", residual=True, out=F32, ref_device="cuda")
     finally:
         cx.lib.call("hv_set_tuning", 16, 0)
