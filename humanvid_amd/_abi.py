@@ -132,10 +132,10 @@ PROTOTYPES = {
     "hv_attention_fp8_quantize": (I, [P, L, P, L, I, I, I, I, P, P, P, P, L, P, L, I, P]),
     "hv_attention_fp8": (I, [C.POINTER(AttentionParams), P, P, P, P, P]),
     "hv_cross_attention": (I, [C.POINTER(CrossAttentionParams), P]),
-    "hv_cross_attention_workspace": (L, [C.POINTER(CrossAttentionParams)]),
+    "hv_cross_attention_workspace": (I, [C.POINTER(CrossAttentionParams), C.POINTER(L)]),
     "hv_fp8_quantize": (I, [P, L, I, I, I, P, L, P, L, L, P]),
     "hv_gemm_fp8": (I, [C.POINTER(GemmFp8Params), P]),
-    "hv_gemm_fp8_workspace": (L, [C.POINTER(GemmFp8Params)]),
+    "hv_gemm_fp8_workspace": (I, [C.POINTER(GemmFp8Params), C.POINTER(L)]),
     "hv_set_tuning": (I, [I, I]),
     "hv_temporal_attention": (I, [C.POINTER(TemporalAttentionParams), P]),
     "hv_pack_ncfhw": (I, [P, I, I, I, I, I, I, P, I, I, P, I, P]),

@@ -133,12 +133,13 @@ int hv_cross_attention(const hv_cross_attention_params* p, void* stream) {
                                   "strides >= 0 in multiples of 8 elements, rows of K and V at most 2^24 elements apart");
     return hv_check_launch("hv_cross_attention");
 }
-long hv_cross_attention_workspace(const hv_cross_attention_params* p) {
-    if (!p) return hv_fail(HV_EINVAL, "hv_cross_attention_workspace: null parameters");
+int hv_cross_attention_workspace(const hv_cross_attention_params* p, long* floats) {
+    if (!p || !floats) return hv_fail(HV_EINVAL, "hv_cross_attention_workspace: null parameters");
     const long n = hvk_cross_attention_workspace(*p);
     if (n == -2) return hv_fail(HV_ENOTSUP, "hv_cross_attention_workspace: head dim must be 40, 64, 80, 128 or 160");
     if (n < 0) return hv_fail(HV_EINVAL, "hv_cross_attention_workspace: need sizes >= 0 and heads a multiple of kv_heads");
-    return n;
+    *floats = n;
+    return HV_OK;
 }
 
 int hv_fp8_quantize(const uint16_t* X, long ldx, int M, int K, int block_rows, uint8_t* Q, long ldq, float* scale, long scale_row,
@@ -158,11 +159,12 @@ int hv_gemm_fp8(const hv_gemm_fp8_params* p, void* stream) {
                                                     "x_scale_row in 0 .. 2^21, rows of Y apart");
     return hv_check_launch("hv_gemm_fp8");
 }
-long hv_gemm_fp8_workspace(const hv_gemm_fp8_params* p) {
-    if (!p) return hv_fail(HV_EINVAL, "hv_gemm_fp8_workspace: null parameters");
+int hv_gemm_fp8_workspace(const hv_gemm_fp8_params* p, long* floats) {
+    if (!p || !floats) return hv_fail(HV_EINVAL, "hv_gemm_fp8_workspace: null parameters");
     const long n = hvk_gemm_fp8_workspace(*p);
     if (n < 0) return hv_fail(HV_EINVAL, "hv_gemm_fp8_workspace: need M, N >= 0 and K a positive multiple of 16");
-    return n;
+    *floats = n;
+    return HV_OK;
 }
 
 static int g_hv_cmdlist_fallbacks = 0;  // command lists whose graph capture failed (hv_cmdlist_fallbacks())

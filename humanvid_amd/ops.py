@@ -216,10 +216,9 @@ def cross_attention(lib, stream, q, k, v, o, *, heads, kv_heads=None, kv_len=Non
         _p(kv_len), _p(key_mask), ms, B, Lq, Lk, heads, KH, D, 1.0 / math.sqrt(D) if scale is None else scale,
         _p(workspace), 0 if workspace is None else workspace.numel())
     if query_workspace:
-        n = lib.cdll.hv_cross_attention_workspace(C.byref(p))
-        if n < 0:
-            lib.check(n)
-        return n
+        n = C.c_long()
+        lib.call("hv_cross_attention_workspace", C.byref(p), C.byref(n))
+        return n.value
     _on_current_device("cross_attention", q, k, v, o, kv_len, key_mask, workspace)
     lib.call("hv_cross_attention", C.byref(p), stream)
 
@@ -275,10 +274,9 @@ def gemm_fp8(lib, stream, x, x_scale, w, w_scale, y, *, bias=None, residual=None
         _p(bias), _p(residual), 0 if residual is None else residual.stride(0), _p(workspace),
         0 if workspace is None else workspace.numel())
     if query_workspace:
-        n = lib.cdll.hv_gemm_fp8_workspace(C.byref(p))
-        if n < 0:
-            lib.check(n)
-        return n
+        n = C.c_long()
+        lib.call("hv_gemm_fp8_workspace", C.byref(p), C.byref(n))
+        return n.value
     _on_current_device("gemm_fp8", x, x_scale, w, w_scale, y, bias, residual, workspace)
     lib.call("hv_gemm_fp8", C.byref(p), stream)
 

@@ -244,7 +244,7 @@ typedef struct hv_cross_attention_params {
     long workspace_floats;
 } hv_cross_attention_params;
 int hv_cross_attention(const hv_cross_attention_params* p, void* stream);
-long hv_cross_attention_workspace(const hv_cross_attention_params* p); /* floats hv_cross_attention needs for these sizes, negative on error */
+int hv_cross_attention_workspace(const hv_cross_attention_params* p, long* floats); /* the scratch hv_cross_attention needs for these sizes */
 
 /* ---- projections in 8-bit floating point (OCP e4m3) with a scale for each block of 128 of the reduction -----------------
  * hv_fp8_quantize: X [M][K] bf16 -> Q [M][K] e4m3 and one scale per block_rows x 128 block (block_rows 1: activations, 128:
@@ -275,7 +275,7 @@ typedef struct hv_gemm_fp8_params {
     long workspace_floats;
 } hv_gemm_fp8_params;
 int hv_gemm_fp8(const hv_gemm_fp8_params* p, void* stream);
-long hv_gemm_fp8_workspace(const hv_gemm_fp8_params* p); /* floats of scratch hv_gemm_fp8 needs for these sizes, negative on error */
+int hv_gemm_fp8_workspace(const hv_gemm_fp8_params* p, long* floats); /* the scratch hv_gemm_fp8 needs for these sizes */
 
 /* kernel-variant selection for A/B measurements (process-global; not needed for correctness) */
 #define HV_TUNE_ATTN_D40 0     /* head dim 40: 0 (default) = the dedicated 8-wave kernel (hv_attention40.h: 32x32x16 QK^T, 256 queries per workgroup); 2 = the generic kernel (A/B) */

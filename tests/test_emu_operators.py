@@ -275,7 +275,7 @@ def test_null_operands_are_refused(cx):
     assert cx.lib.cdll.hv_cross_attention(None, None) == A.HV_EINVAL
     p.Lq = -1
     assert cx.lib.cdll.hv_cross_attention(C.byref(p), None) == A.HV_EINVAL
-    assert cx.lib.cdll.hv_cross_attention_workspace(C.byref(p)) == A.HV_EINVAL
+    assert cx.lib.cdll.hv_cross_attention_workspace(C.byref(p), C.byref(C.c_long())) == A.HV_EINVAL
     for field, value in (("ldq", -8), ("k_stride_b", -40), ("ldk", 1 << 25), ("mask_stride_b", -1)):
         buf = torch.zeros(64, dtype=BF16)
         p = A.CrossAttentionParams(B=1, Lq=1, Lk=1, heads=1, kv_heads=1, D=40, scale=1.0, Q=buf.data_ptr(), K=buf.data_ptr(), V=buf.data_ptr(),
