@@ -187,13 +187,14 @@ def cross_attention(lib, stream, q, k, v, o, *, heads, kv_heads=None, kv_len=Non
     expanded over the batch); heads // kv_heads query heads share a key head.  kv_len int32 [B], key_mask uint8 / bool [B, Lk] on the
     device.  An entry that attends to nothing gets zeros.  scale: 1 / sqrt(D) by default.  o may be q, and overlap nothing else.
     query_workspace=True launches nothing and returns the fp32 elements `workspace` needs for these sizes (0: none)."""
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or o.shape != q.shape:
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or v.shape != ks or o.shape != qs:
         raise ValueError("cross_attention: q, o [B, Lq, heads * D] and k, v [B, Lk, kv_heads * D] expected")
-    B, Lq, Cq = q.shape
-    Lk = k.shape[1]
+    B, Lq, Cq = qs
+    Bk, Lk, Ck = ks
     KH = heads if kv_heads is None else kv_heads
-    if heads <= 0 or KH <= 0 or Cq % heads or k.shape[0] != B or k.shape[2] != Cq // heads * KH:
-        raise ValueError(f"cross_attention: q {tuple(q.shape)}, k {tuple(k.shape)} do not fit {heads} heads, {KH} key heads")
+    if heads <= 0 or KH <= 0 or Cq % heads or Bk != B or Ck != Cq // heads * KH:
+        raise ValueError(f"cross_attention: q {tuple(qs)}, k {tuple(ks)} do not fit {heads} heads, {KH} key heads")
     if q.dtype != BF16 or k.dtype != BF16 or v.dtype != BF16 or o.dtype != BF16:
         raise ValueError("cross_attention: q, k, v, o must be bfloat16")
     D = Cq // heads
@@ -251,16 +252,19 @@ def gemm_fp8(lib, stream, x, x_scale, w, w_scale, y, *, bias=None, residual=None
     [M, ceil(K / 128)], w_scale [ceil(N / 128), ceil(K / 128)] fp32 (any strides), y bf16 or fp32, bias fp32 [N], residual bf16 [M, N]
     (may be y).  K a multiple of 16; x / w / y / residual may be row-strided views.
     query_workspace=True launches nothing and returns the fp32 elements `workspace` needs for these sizes (0: none)."""
-    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or y.shape != (x.shape[0], w.shape[0]):
+    xsh, wsh = x.shape, w.shape
+    if len(xsh) != 2 or len(wsh) != 2 or xsh[1] != wsh[1] or y.shape != (xsh[0], wsh[0]):
         raise ValueError("gemm_fp8: x [M, K], w [N, K], y [M, N] expected")
-    M, K = x.shape
-    N = w.shape[0]
+    M, K = xsh
+    N = wsh[0]
     kb = -(-K // 128)
-    if x.dtype not in FP8 or w.dtype not in FP8 or y.dtype not in (BF16, torch.float32):
+    out_f32 = y.dtype == torch.float32
+    if x.dtype not in FP8 or w.dtype not in FP8 or not (out_f32 or y.dtype == BF16):
         raise ValueError("gemm_fp8: x, w float8_e4m3fn or uint8, y bfloat16 or float32 expected")
     if x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32 or x_scale.shape != (M, kb) or w_scale.shape != (-(-N // 128), kb):
         raise ValueError(f"gemm_fp8: float32 x_scale {(M, kb)} and w_scale {(-(-N // 128), kb)} expected, got {tuple(x_scale.shape)}, {tuple(w_scale.shape)}")
-    if (K > 1 and (x.stride(1) != 1 or w.stride(1) != 1)) or (N > 1 and y.stride(1) != 1) or (M > 1 and y.stride(0) < N):
+    (ldx, x1), (ldw, w1), (ldy, y1), (xs0, xs1), (ws0, ws1) = x.stride(), w.stride(), y.stride(), x_scale.stride(), w_scale.stride()
+    if (K > 1 and (x1 != 1 or w1 != 1)) or (N > 1 and y1 != 1) or (M > 1 and ldy < N):
         raise ValueError("gemm_fp8: the rows of x, w and y must be contiguous, those of y must not overlap")
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or not bias.is_contiguous()):
         raise ValueError("gemm_fp8: bias must be contiguous float32 [N]")
@@ -269,8 +273,7 @@ def gemm_fp8(lib, stream, x, x_scale, w, w_scale, y, *, bias=None, residual=None
     if workspace is not None and (workspace.dtype != torch.float32 or not workspace.is_contiguous()):
         raise ValueError("gemm_fp8: workspace must be contiguous float32")
     p = A.GemmFp8Params(
-        x.data_ptr(), x.stride(0), x_scale.data_ptr(), x_scale.stride(0), x_scale.stride(1), w.data_ptr(), w.stride(0),
-        w_scale.data_ptr(), w_scale.stride(0), w_scale.stride(1), y.data_ptr(), y.stride(0), y.dtype == torch.float32, M, N, K,
+        x.data_ptr(), ldx, x_scale.data_ptr(), xs0, xs1, w.data_ptr(), ldw, w_scale.data_ptr(), ws0, ws1, y.data_ptr(), ldy, out_f32, M, N, K,
         _p(bias), _p(residual), 0 if residual is None else residual.stride(0), _p(workspace),
         0 if workspace is None else workspace.numel())
     if query_workspace:
