@@ -222,6 +222,9 @@ class UNet3DEngine:
         gets to_out's bias)."""
         if ehs.ndim != 3 or ehs.shape[1] < 1:
             raise ValueError(f"encoder_hidden_states: [batch, tokens, channels] with at least one token expected, got {tuple(ehs.shape)}")
+        width = self.w[self.locations[0] + ".transformer_blocks.0.attn2.to_v.w"].shape[1] if self.locations else ehs.shape[2]
+        if ehs.shape[2] != width:
+            raise ValueError(f"encoder_hidden_states: {width} channels expected, got {ehs.shape[2]}")
         if mask is not None and tuple(mask.shape) != tuple(ehs.shape[:2]):
             raise ValueError(f"encoder_attention_mask: {tuple(ehs.shape[:2])} expected, got {tuple(mask.shape)}")
         B = ehs.shape[0]

@@ -65,6 +65,9 @@ def test_states_refusals_and_the_way_back(engine):
         eng.set_encoder_hidden_states(e[0])
     with pytest.raises(ValueError):
         eng.set_encoder_hidden_states(e[:, :0])
+    for tokens in (1, 4):
+        with pytest.raises(ValueError, match="768 channels"):
+            eng.set_encoder_hidden_states(e[:, :tokens, :512])
     with pytest.raises(ValueError):
         eng.set_encoder_hidden_states(e, torch.ones(2, 5))
     eng.set_encoder_hidden_states(e)
