@@ -180,3 +180,13 @@ def test_two_streams_at_once(cx):
     torch.cuda.synchronize()
     for t, w in zip((a, b), want):
         assert torch.equal(t["o"], w[0]) and torch.equal(t["y"], w[1])
+
+
+def test_current_stream_is_torchs():
+    from humanvid_amd import lib
+
+    side = torch.cuda.Stream()
+    assert lib.current_stream() == torch.cuda.current_stream().cuda_stream
+    with torch.cuda.stream(side):
+        assert lib.current_stream() == side.cuda_stream == torch.cuda.current_stream().cuda_stream
+    assert lib.current_stream() == torch.cuda.current_stream().cuda_stream
