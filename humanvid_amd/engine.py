@@ -65,7 +65,7 @@ class UNet3DEngine:
         self.bank_version = None
         self.cross_const: Dict[str, torch.Tensor] = {}
         self.cross_kv: Dict[str, torch.Tensor] = {}  # encoder states of several tokens: [batch entries][tokens][keys | values] per transformer
-        self.cross_mask: Optional[torch.Tensor] = None  # [batch entries][tokens] uint8 or None: every token
+        self._cross_shared: Dict[str, Optional[torch.Tensor]] = {"mask": None}  # the states' token mask (cross_mask)
         self.do_cfg = True
         # spatial attention on the fp8 (e4m3) MFMA -- hv_attention_fp8 (transposed-V kernel family)
         # (denoising UNet only: the ReferenceNet write pass runs once per clip and keeps its banks at bf16 precision)
@@ -91,10 +91,21 @@ class UNet3DEngine:
     def stream(self) -> int:
         return hvlib.current_stream()
 
+    @property
+    def cross_mask(self) -> Optional[torch.Tensor]:
+        """[batch entries][tokens] uint8 or None: every token.  Kept in a table as the states' keys | values (cross_kv) are, so that
+        the executors of the halves never hold the states of one call with the mask of another."""
+        return self._cross_shared["mask"]
+
+    @cross_mask.setter
+    def cross_mask(self, mask: Optional[torch.Tensor]):
+        self._cross_shared["mask"] = mask
+
     def clone_for_half(self, half: int, ws: "Workspace | None" = None) -> "UNet3DEngine":
         """An executor for ONE CFG half (batch entry `half` of [unconditional, conditional]) with its own workspace and
-        statistics tables, sharing the packed weights, the projected reference banks and the folded cross-attention
-        constants of this one (read-only during a step).  Make the clones after the banks / embeddings are set.
+        statistics tables, sharing the packed weights, the projected reference banks and what the encoder states became (the folded
+        cross-attention constants, or keys | values and mask) of this one (read-only during a step).  Make the clones after the banks
+        are set; encoder states set later reach them too.
         `ws`: a workspace kept by the caller across calls (the pipeline caches one per half and stream, so that repeated
         denoise() calls do not re-allocate gigabytes on freshly drawn side streams)."""
         import copy
