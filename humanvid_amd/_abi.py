@@ -118,6 +118,7 @@ _STRUCTS = (GemmParams, Conv3x3Params, GroupNormParams, AttentionParams, Tempora
 PROTOTYPES = {
     "hv_last_error": (C.c_char_p, []),
     "hv_abi_version": (I, []),
+    "hv_on_host": (I, []),
     "hv_struct_sizes": (I, [C.POINTER(I), I]),
     "hv_gemm": (I, [C.POINTER(GemmParams), P]),
     "hv_conv3x3": (I, [C.POINTER(Conv3x3Params), P]),
@@ -187,6 +188,7 @@ class HvLibrary:
         mine = [C.sizeof(s) for s in _STRUCTS]
         if n != len(mine) or list(sizes[:n]) != mine:
             raise HvError(f"ABI mismatch between {path} and humanvid_amd/_abi.py: {list(sizes[:n])} vs {mine}")
+        self.host = bool(self.cdll.hv_on_host())  # the host build of the kernels (CPU tests): operands in host memory
 
     def check(self, rc: int):
         if rc == HV_OK:

@@ -35,6 +35,14 @@ extern "C" {
 const char* hv_last_error(void) { return g_err; }
 int hv_abi_version(void) { return 2; }  // 2: gn_part fields, hv_groupnorm_from_parts (round 3)
 
+int hv_on_host(void) {
+#ifdef HV_EMU
+    return 1;
+#else
+    return 0;
+#endif
+}
+
 int hv_struct_sizes(int* out, int capacity) {
     const int s[] = {(int)sizeof(hv_gemm_params),      (int)sizeof(hv_conv3x3_params),
                      (int)sizeof(hv_groupnorm_params), (int)sizeof(hv_attention_params),

@@ -161,12 +161,14 @@ def attention_fp8(lib, stream, q, k, vt, o, kscale, vamax, *, n_images, heads, D
     lib.call("hv_attention_fp8", C.byref(p), _p(kscale), _p(vamax), _p(kscale2), _p(vamax2), stream)
 
 
-def _on_current_device(what, first, *others):
-    """the launch goes to the current device: every tensor has to be there"""
+def _on_current_device(lib, what, first, *others):
+    """the launch goes to the current device: every tensor has to be there (in host memory for the host build of the kernels, and only there)"""
     dev = first.get_device()
     for t in others:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+    if (dev < 0) != lib.host:
+        raise ValueError(f"{what}: tensors on {first.device}, {'host' if lib.host else 'GPU'} memory expected")
     if dev >= 0 and dev != torch.cuda.current_device():
         raise ValueError(f"{what}: tensors on {first.device}, the current device is {torch.cuda.current_device()}")
 
@@ -220,7 +222,7 @@ def cross_attention(lib, stream, q, k, v, o, *, heads, kv_heads=None, kv_len=Non
         n = C.c_long()
         lib.call("hv_cross_attention_workspace", C.byref(p), C.byref(n))
         return n.value
-    _on_current_device("cross_attention", q, k, v, o, kv_len, key_mask, workspace)
+    _on_current_device(lib, "cross_attention", q, k, v, o, kv_len, key_mask, workspace)
     lib.call("hv_cross_attention", C.byref(p), stream)
 
 
@@ -242,7 +244,7 @@ def fp8_quantize(lib, stream, x, q, scale, *, block_rows=1):
         raise ValueError("fp8_quantize: the rows of x and q must be contiguous, those of q must not overlap")
     if _overlaps(scale.shape[0], scale.stride(0), scale.shape[1], scale.stride(1), 1):
         raise ValueError("fp8_quantize: the elements of scale must not overlap")
-    _on_current_device("fp8_quantize", x, q, scale)
+    _on_current_device(lib, "fp8_quantize", x, q, scale)
     lib.call("hv_fp8_quantize", x.data_ptr(), x.stride(0), M, K, block_rows, q.data_ptr(), q.stride(0), scale.data_ptr(),
              scale.stride(0), scale.stride(1), stream)
 
@@ -280,7 +282,7 @@ def gemm_fp8(lib, stream, x, x_scale, w, w_scale, y, *, bias=None, residual=None
         n = C.c_long()
         lib.call("hv_gemm_fp8_workspace", C.byref(p), C.byref(n))
         return n.value
-    _on_current_device("gemm_fp8", x, x_scale, w, w_scale, y, bias, residual, workspace)
+    _on_current_device(lib, "gemm_fp8", x, x_scale, w, w_scale, y, bias, residual, workspace)
     lib.call("hv_gemm_fp8", C.byref(p), stream)
 
 

@@ -33,6 +33,8 @@ extern "C" {
 
 const char* hv_last_error(void);
 int hv_abi_version(void);
+/* 0: this library launches on the GPU and takes device pointers; 1: the host build of the kernels that the CPU tests load */
+int hv_on_host(void);
 /* sizeof() of every parameter struct, in declaration order -- lets a binding verify its mirror */
 int hv_struct_sizes(int* out, int capacity);
 
