@@ -14,7 +14,9 @@
 // operand of the second product if its reduction index runs over the keys in that order (k = 8 g + e is key 4 g + e of the
 // first tile for e < 4, of the second for e >= 4); V is stored row-major in LDS and read transposed in the same order.
 // A masked key's row of K and V is zero in LDS (whatever memory holds there) and its score starts at -inf: the accumulator of
-// the first product is initialised with the chunk's bias (0 / -inf) instead of zero, so masks cost no instruction.
+// the first product is initialised with the chunk's bias (0 / -inf) instead of zero, so masks cost no instruction.  (A query that holds
+// NaN or infinity makes such a score NaN and spoils its row, as its attended states' scores do anyway.  Chunks without an attended
+// state are passed over, so that an entry without any gives zeros whatever its queries hold.)
 // Query heads that share a key head are rows of the same tile: row r of a (batch, key head) is query r / G, head r % G.
 #pragma once
 #include "hv_common.h"
@@ -173,13 +175,21 @@ __global__ __launch_bounds__(256, D == 40 ? 3 : 2) void hv_cross_attention_few_k
         const uint8_t* mask = p.key_mask ? p.key_mask + (long)b * p.mask_stride_b : nullptr;
         unsigned char* const part = smem + wave * VPART;
         constexpr int VP = DT * 2;  // pieces of a padded V row
+        bool some = false;
 #pragma unroll
         for (int kt = 0; kt < NT; ++kt) {
             const int row = kt * 16 + col;
             const bool on = row < len && (mask == nullptr || mask[row] != 0);
+            some = some || on;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
                 kf[kt][ks] = hv_as_bf16x8(on && ks * 32 + g * 8 < D ? hv_ld16(Kb + (long)row * p.ldk + ks * 32 + g * 8) : zero4);
+        }
+        if (hv_ballot(some) == 0) {  // (the same in all four waves) nothing attended: zeros, the queries are not looked at
+            const int q0 = group * a.per_wg * TQ, queries = min(a.per_wg * TQ, p.Lq - q0);
+            bf16_t* const O = p.O + (long)b * p.o_stride_b + (long)q0 * p.ldo + (long)hgroup * 4 * D;
+            for (long i = tid; i < (long)queries * NPC; i += 256) hv_st16(O + i / NPC * p.ldo + i % NPC * 8, zero4);
+            return;
         }
 #pragma unroll
         for (int pr = 0; pr < NP; ++pr) {
@@ -446,6 +456,7 @@ __global__ __launch_bounds__(256, QT == 1 && D < 128 ? 3 : 2) void hv_cross_atte
             bias = sBias[1 + (ch & 1)] + g * 4;
             if (tid < CH) sBias[1 + (ch & 1)][tid] = keep >> tid & 1ul ? 0.f : -INFINITY;
             hv_barrier_raw();
+            if (keep == 0) continue;  // (the same in all four waves)
         }
         f32x4 s[QT][KT];
         u32x4 kv[2][KS];  // the next 16 keys' operands are read while this 16's are used; fences keep it at that
@@ -618,6 +629,7 @@ __global__ __launch_bounds__(256, 2) void hv_cross_attention_rows_kernel(HvCross
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[t][e] = keep >> (t * 16 + g * 4 + e) & 1u ? 0.f : -INFINITY;
+            if (keep == 0) continue;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
                 s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv_as_bf16x8(on[t] ? kreg[t][ks] : zero4), qf[ks], s[t], 0, 0, 0);

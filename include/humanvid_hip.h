@@ -222,9 +222,9 @@ int hv_attention_fp8(const hv_attention_params* p, const float* kscale, const fl
 /* ---- cross attention: Lq queries per batch entry to Lk encoder states ------------------------------------------------
  * The UNets' attn2 when encoder_hidden_states has more than one token (src/models/attention.py:410-424, diffusers Attention):
  * O[b][i][h] = sum_j softmax_j(scale Q[b][i][h] . K[b][j][g]) V[b][j][g],  g = h / (heads / kv_heads), over the attended states:
- * j < kv_len[b] and key_mask[b][j] != 0.  A batch entry with no attended state gets zeros; what memory holds in the other
- * states (NaN included) does not reach the output, and states at or behind kv_len are not read.  Values are row-major.  All frames of a
- * clip that share their half's prompt are ONE batch entry (Lq = frames * tokens).  O may be Q, and overlap nothing else.  Any Lq, Lk >= 0; D in
+ * j < kv_len[b] and key_mask[b][j] != 0.  A batch entry with no attended state gets zeros, whatever its queries hold; what memory
+ * holds in the other states (NaN included) does not reach the output, and states at or behind kv_len are not read.  A query that holds
+ * NaN or infinity spoils its own row only.  Values are row-major.  All frames of a clip that share their half's prompt are ONE batch entry (Lq = frames * tokens).  O may be Q, and overlap nothing else.  Any Lq, Lk >= 0; D in
  * {40, 64, 80, 128, 160}; pointers 16-byte aligned, strides >= 0 in multiples of 8 elements (the batch strides of K, V and the mask may be 0:
  * shared states; rows of K and V at most 2^24 elements apart).  The keys are cut into ranges that are joined by a second launch where the queries alone would not fill the
  * chip: hv_cross_attention_workspace() floats of scratch, not to be shared by calls that may run at the same time. */

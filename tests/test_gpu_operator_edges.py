@@ -1,0 +1,19 @@
+"""The cross attention and 8-bit projection operators at values that are not numbers, on a real MI355X."""
+import pytest
+
+import operator_edge_cases as ec
+from test_gpu_operators import cx  # noqa: F401  (the fixture)
+
+pytestmark = pytest.mark.gpu
+SIZES = ec.CROSS_KERNELS + [(1000, 77, 8, 2, 40), (300, 700, 8, 8, 160), (8, 4109, 16, 4, 128), (200, 3000, 4, 4, 80)]
+
+
+@pytest.mark.parametrize("how", ["len", "mask", "part"])
+@pytest.mark.parametrize("Lq,Lk,heads,kv_heads,D", SIZES)
+def test_empty_entries_are_zero_whatever_they_hold(cx, Lq, Lk, heads, kv_heads, D, how):  # noqa: F811
+    ec.case_empty_entries(cx, Lq, Lk, heads, kv_heads, D, how, seed=Lk)
+
+
+@pytest.mark.parametrize("Lq,Lk,heads,kv_heads,D", SIZES)
+def test_masks_that_leave_whole_stretches_out(cx, Lq, Lk, heads, kv_heads, D):  # noqa: F811
+    ec.case_masked_stretches(cx, Lq, Lk, heads, kv_heads, D, seed=Lk)
