@@ -305,7 +305,9 @@ class UNet3DEngine:
                  colsum=w[t + ".attn2.q.colsum"])
         qb, ob, kw = q.view(B, M // B, C), o.view(B, M // B, C), dict(heads=self.heads, key_mask=mask)
         n = ops.cross_attention(L, st, qb, kv[..., :C], kv[..., C:], ob, query_workspace=True, **kw)
-        ops.cross_attention(L, st, qb, kv[..., :C], kv[..., C:], ob, workspace=ws.get("tr_xws", (n,), F32) if n else None, **kw)
+        # (one buffer a level: a buffer for all of them would move where a later level asks for more, under a recording of the earlier)
+        work = ws.get(f"tr_xws_{M}x{C}", (n,), F32) if n else None
+        ops.cross_attention(L, st, qb, kv[..., :C], kv[..., C:], ob, workspace=work, **kw)
         self.run.gemm_ln(o, w[t + ".attn2.to_out.0.w"], hid, bias=w[t + ".attn2.to_out.0.bias"], residual=hid)
 
     def set_reference_banks(self, banks: Optional[Dict[str, torch.Tensor]], do_cfg: bool):

@@ -46,3 +46,57 @@ def test_half_executors_see_new_states_and_their_mask(engine, before, after):  #
         assert torch.equal(_attend(e, h[i:i + 1])[0], want[i]), i
     eng.set_encoder_hidden_states(torch.randn(2, 1, 768, generator=g))  # one token: no states, no mask, in any of them
     assert all(not e.cross_kv and e.cross_mask is None for e in (eng, *halves))
+
+
+def test_a_recorded_step_keeps_its_scratch(engine, monkeypatch):  # noqa: F811
+    """recorded without an eager pass before it: the scratch that one level's launches were recorded with is still there when another
+    level has asked for more, and the replay computes what an eager pass does"""
+    import ctypes
+
+    from humanvid_amd import engine as E
+
+    eng, sd, cfg = engine
+    g = torch.Generator().manual_seed(13)
+    tokens = 1100  # few queries, many states: ranges, joined through scratch
+    shared = eng
+    eng = _half(eng, 0)
+    eng.cfg_half = None  # the whole batch, with a workspace that nothing has used
+    levels = [("down_blocks.0.attentions.0", 320), ("mid_block.attentions.0", cfg["block_out_channels"][-1])]
+    assert levels[1][1] > 320
+    eng.locations = [loc for loc, _ in levels]
+    eng.set_encoder_hidden_states(torch.randn(2, 2, 768, generator=g))  # (their weights)
+    for loc, C in levels:  # what the projection of many tokens would leave here, without its time on the emulator
+        eng.cross_kv[loc] = torch.randn(2, tokens, 2 * C, generator=g).to(BF16)
+    hid = {loc: torch.randn(2 * ROWS, C, generator=g).to(BF16) for loc, C in levels}
+    used, call = [], E.ops.cross_attention
+
+    def logged(*a, workspace=None, **kw):
+        if workspace is not None:
+            used.append((workspace.data_ptr(), workspace.numel()))
+        return call(*a, workspace=workspace, **kw)
+
+    monkeypatch.setattr(E.ops, "cross_attention", logged)
+    h = ctypes.c_void_p()
+    eng.lib.call("hv_cmdlist_begin")
+    try:
+        for loc, _ in levels:
+            eng._cross_attention(loc, hid[loc], 2)
+    finally:
+        eng.lib.call("hv_cmdlist_end", ctypes.byref(h))
+    try:
+        assert len(used) == 2 and used[0][1] < used[1][1]
+        held = [(t.data_ptr(), t.numel()) for t in eng.ws.bufs.values()]
+        for at, n in used:
+            assert any(p <= at and at + 4 * n <= p + 4 * m for p, m in held), "scratch of the recording was let go"
+        for kv in eng.cross_kv.values():  # new states in the same buffers
+            kv.copy_(torch.randn(kv.shape, generator=g))
+        want = {loc: torch.randn(t.shape, generator=g).to(BF16) for loc, t in hid.items()}
+        for loc, t in hid.items():
+            t.copy_(want[loc])
+        eng.lib.call("hv_cmdlist_run", h, None)
+        for loc, t in hid.items():
+            eng._cross_attention(loc, want[loc], 2)
+            assert torch.equal(t, want[loc]), loc
+    finally:
+        eng.lib.call("hv_cmdlist_destroy", h)
+        shared.cross_kv.clear()
