@@ -58,6 +58,7 @@ class UNet3DEngine:
         self.ws = Workspace(self.device)
         self.shard = shard
         self.heads = self.cfg["attention_head_dim"]
+        self.cross_width: Optional[int] = None  # channels of the encoder states
         self.groups = self.cfg["norm_num_groups"]
         self.eps = self.cfg["norm_eps"]
         self.w: Dict[str, torch.Tensor] = {}
@@ -188,6 +189,7 @@ class UNet3DEngine:
                         [sd[t + ".attn1.to_k.weight"], sd[t + ".attn1.to_v.weight"]], dim=0).float()))
                     lin(t + ".attn1.to_out.0")
                     lin(t + ".attn2.to_v", bias=False)
+                    self.cross_width = sd[t + ".attn2.to_v.weight"].shape[1]
                     lin(t + ".attn2.to_out.0")
                     lnfold(t + ".ff1", sd[t + ".ff.net.0.proj.weight"], sd[t + ".ff.net.0.proj.bias"], t + ".norm3",
                            geglu=True)
@@ -227,15 +229,14 @@ class UNet3DEngine:
 
     # ------------------------------------------------------------------------------------------
     def set_encoder_hidden_states(self, ehs: torch.Tensor, mask: Optional[torch.Tensor] = None):
-        """ehs [B, L, 768], one row of states per batch entry.  L == 1 without a mask: fold the one-key cross-attention of every
+        """ehs [B, L, channels], one row of states per batch entry.  L == 1 without a mask: fold the one-key cross-attention of every
         transformer into a per-batch constant (attention.py:410-424 -> to_out(to_v(e)) + bias).  Otherwise: project the states to
         keys | values; the transformers attend to them, to the tokens only where mask [B, L] is non-zero (an entry without any token
         gets to_out's bias)."""
         if ehs.ndim != 3 or ehs.shape[1] < 1:
             raise ValueError(f"encoder_hidden_states: [batch, tokens, channels] with at least one token expected, got {tuple(ehs.shape)}")
-        width = self.w[self.locations[0] + ".transformer_blocks.0.attn2.to_v.w"].shape[1] if self.locations else ehs.shape[2]
-        if ehs.shape[2] != width:
-            raise ValueError(f"encoder_hidden_states: {width} channels expected, got {ehs.shape[2]}")
+        if self.cross_width is not None and ehs.shape[2] != self.cross_width:
+            raise ValueError(f"encoder_hidden_states: {self.cross_width} channels expected, got {ehs.shape[2]}")
         if mask is not None and tuple(mask.shape) != tuple(ehs.shape[:2]):
             raise ValueError(f"encoder_attention_mask: {tuple(ehs.shape[:2])} expected, got {tuple(mask.shape)}")
         B = ehs.shape[0]
@@ -245,7 +246,7 @@ class UNet3DEngine:
             return
         self.cross_kv.clear()
         self.cross_mask = None
-        e = self._dev(ehs[:, 0], BF16)
+        e = self._packed_states(ehs)
         for loc in self.locations:
             t = loc + ".transformer_blocks.0"
             C = self.w[t + ".attn2.to_out.0.w"].shape[0]
@@ -256,6 +257,12 @@ class UNet3DEngine:
                 c = torch.empty(B, C, dtype=F32, device=self.device)
                 self.cross_const[loc] = c
             ops.gemm(self.lib, st, v, self.w[t + ".attn2.to_out.0.w"], c, bias=self.w[t + ".attn2.to_out.0.bias"])
+
+    def _packed_states(self, ehs: torch.Tensor) -> torch.Tensor:
+        """[B, L, channels] -> [B * L, channels up to a multiple of 64, as the packed weights have], bf16 on the device, zeros behind"""
+        e = self._dev(ehs.reshape(-1, ehs.shape[2]), BF16)
+        pad = packing.round_up(e.shape[1], 64) - e.shape[1]
+        return torch.nn.functional.pad(e, (0, pad)) if pad else e
 
     def _set_cross_states(self, ehs: torch.Tensor, mask: Optional[torch.Tensor]):
         B, tokens, _ = ehs.shape
@@ -269,7 +276,7 @@ class UNet3DEngine:
                 self.w[t + ".attn2.q.colsum"], self.w[t + ".attn2.q.bias"] = self._dev(colsum, F32), self._dev(bf, F32)
                 self.w[t + ".attn2.kv.w"] = self._dev(packing.pack_linear(torch.cat(
                     [sd[t + ".attn2.to_k.weight"], sd[t + ".attn2.to_v.weight"]], dim=0).float()))
-        x = self._dev(ehs.reshape(B * tokens, -1), BF16)
+        x = self._packed_states(ehs)
         old = dict(self.cross_kv)
         self.cross_kv.clear()  # (in place: executors of one half share the table)
         for loc in self.locations:

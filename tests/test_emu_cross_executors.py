@@ -64,7 +64,7 @@ def test_a_recorded_step_keeps_its_scratch(engine, monkeypatch):  # noqa: F811
     levels = [("down_blocks.0.attentions.0", 320), ("mid_block.attentions.0", cfg["block_out_channels"][-1])]
     assert levels[1][1] > 320
     eng.locations = [loc for loc, _ in levels]
-    eng.set_encoder_hidden_states(torch.randn(2, 2, 768, generator=g))  # (their weights)
+    shared.set_encoder_hidden_states(torch.randn(2, 2, 768, generator=g))  # (their weights)
     for loc, C in levels:  # what the projection of many tokens would leave here, without its time on the emulator
         eng.cross_kv[loc] = torch.randn(2, tokens, 2 * C, generator=g).to(BF16)
     hid = {loc: torch.randn(2 * ROWS, C, generator=g).to(BF16) for loc, C in levels}
@@ -100,3 +100,38 @@ def test_a_recorded_step_keeps_its_scratch(engine, monkeypatch):  # noqa: F811
     finally:
         eng.lib.call("hv_cmdlist_destroy", h)
         shared.cross_kv.clear()
+
+
+def test_states_narrower_than_the_packed_weights():
+    """a model whose encoder states have 96 channels (its packed weights are padded to 128): one token and several"""
+    from test_emu_engine import O, _engine_on_emulator
+    from humanvid_amd.unet3d import UNet3DConditionModel
+
+    cfg = O.tiny_unet3d_cfg(cross_attention_dim=96)
+    sd = O.make_unet3d_weights(cfg, seed=2)
+    net = UNet3DConditionModel(**dict(cfg, use_inflated_groupnorm=True, unet_use_cross_frame_attention=False,
+                                      unet_use_temporal_attention=False, motion_module_type="Vanilla"))
+    net.load_state_dict(sd, strict=True)
+    eng, (hvlib, restore) = _engine_on_emulator(net)
+    try:
+        eng.locations = [LOC]
+        t = LOC + ".transformer_blocks.0"
+        heads = cfg["attention_head_dim"]
+        g = torch.Generator().manual_seed(17)
+        e = torch.randn(2, 3, 96, generator=g)
+        eng.set_encoder_hidden_states(e[:, :1])
+        want = torch.nn.functional.linear(torch.nn.functional.linear(e[:, 0], sd[t + ".attn2.to_v.weight"]),
+                                          sd[t + ".attn2.to_out.0.weight"], sd[t + ".attn2.to_out.0.bias"])
+        assert float((eng.cross_const[LOC].float() - want).norm() / want.norm()) < 1e-2  # bf16 weights and states
+        eng.set_encoder_hidden_states(e)
+        h = torch.randn(2, ROWS, 320, generator=g).to(BF16)
+        got = _attend(eng, h)
+        for b in range(2):
+            want = h[b:b + 1].float() + O.attention(sd, t + ".attn2", O.layer_norm(sd, t + ".norm2", h[b:b + 1].float()), e[b:b + 1], heads)
+            assert float((got[b].float() - want[0]).norm() / want.norm()) < 1e-2
+        for width in (64, 128):
+            for tokens in (1, 3):
+                with pytest.raises(ValueError, match="96 channels"):
+                    eng.set_encoder_hidden_states(torch.randn(2, tokens, width, generator=g))
+    finally:
+        hvlib.current_stream = restore
