@@ -138,14 +138,14 @@ int hv_cross_attention(const hv_cross_attention_params* p, void* stream) {
     if (rc == -3) return hv_fail(HV_EINVAL, "hv_cross_attention: workspace smaller than hv_cross_attention_workspace() floats");
     if (rc != 0)
         return hv_fail(HV_EINVAL, "hv_cross_attention: need sizes >= 0, heads a multiple of kv_heads, a scale in (0, 1e30], 16-byte aligned pointers, "
-                                  "strides >= 0 in multiples of 8 elements, rows of K and V at most 2^24 elements apart");
+                                  "strides >= 0 in multiples of 8 elements, rows of K and V at most 2^24 elements apart, at most 2^30 states, less than 2^32 threads");
     return hv_check_launch("hv_cross_attention");
 }
 int hv_cross_attention_workspace(const hv_cross_attention_params* p, long* floats) {
     if (!p || !floats) return hv_fail(HV_EINVAL, "hv_cross_attention_workspace: null parameters");
     const long n = hvk_cross_attention_workspace(*p);
     if (n == -2) return hv_fail(HV_ENOTSUP, "hv_cross_attention_workspace: head dim must be 40, 64, 80, 128 or 160");
-    if (n < 0) return hv_fail(HV_EINVAL, "hv_cross_attention_workspace: need sizes >= 0 and heads a multiple of kv_heads");
+    if (n < 0) return hv_fail(HV_EINVAL, "hv_cross_attention_workspace: need sizes >= 0, heads a multiple of kv_heads, at most 2^30 states, less than 2^32 threads");
     *floats = n;
     return HV_OK;
 }
@@ -154,7 +154,8 @@ int hv_fp8_quantize(const uint16_t* X, long ldx, int M, int K, int block_rows, u
                     long scale_k, void* stream) {
     if (M > 0 && (!X || !Q || !scale)) return hv_fail(HV_EINVAL, "hv_fp8_quantize: null operand");
     if (hvk_fp8_quantize(X, ldx, M, K, block_rows, Q, ldq, scale, scale_row, scale_k, (hipStream_t)stream) != 0)
-        return hv_fail(HV_EINVAL, "hv_fp8_quantize: need M >= 0, K a positive multiple of 16, block_rows 1 or 128, 16-byte aligned rows, rows of Q apart");
+        return hv_fail(HV_EINVAL, "hv_fp8_quantize: need M >= 0, K a positive multiple of 16, block_rows 1 or 128, 16-byte aligned rows, rows of Q apart, "
+                                  "less than 2^32 threads (16 for a block of one row), at most 65535 row blocks of 128");
     return hv_check_launch("hv_fp8_quantize");
 }
 
@@ -164,13 +165,13 @@ int hv_gemm_fp8(const hv_gemm_fp8_params* p, void* stream) {
     const int rc = hvk_gemm_fp8(*p, (hipStream_t)stream);
     if (rc == -3) return hv_fail(HV_EINVAL, "hv_gemm_fp8: workspace smaller than hv_gemm_fp8_workspace() floats");
     if (rc != 0) return hv_fail(HV_EINVAL, "hv_gemm_fp8: need M, N >= 0, K a positive multiple of 16, X and W rows 16-byte aligned with strides up to 8 MiB, "
-                                                    "x_scale_row in 0 .. 2^21, rows of Y apart");
+                                                    "x_scale_row in 0 .. 2^21, rows of Y apart, less than 2^32 threads");
     return hv_check_launch("hv_gemm_fp8");
 }
 int hv_gemm_fp8_workspace(const hv_gemm_fp8_params* p, long* floats) {
     if (!p || !floats) return hv_fail(HV_EINVAL, "hv_gemm_fp8_workspace: null parameters");
     const long n = hvk_gemm_fp8_workspace(*p);
-    if (n < 0) return hv_fail(HV_EINVAL, "hv_gemm_fp8_workspace: need M, N >= 0 and K a positive multiple of 16");
+    if (n < 0) return hv_fail(HV_EINVAL, "hv_gemm_fp8_workspace: need M, N >= 0, K a positive multiple of 16, less than 2^32 threads");
     *floats = n;
     return HV_OK;
 }

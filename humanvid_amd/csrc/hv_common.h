@@ -279,6 +279,8 @@ extern thread_local char g_hv_note[192];
         if (g_hv_prof) snprintf(g_hv_note, sizeof(g_hv_note), __VA_ARGS__); \
     } while (0)
 
+static inline bool hv_fits_launch(long groups, int threads) { return groups * threads <= 0xffffffffL; }  // threads of a launch: 32 bits
+
 template <class... KArgs, class... Args>
 static inline void hv_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, hipStream_t stream, Args... args) {
 #ifdef HV_EMU

@@ -760,7 +760,7 @@ static inline int hv_cross_attention_plan(const hv_cross_attention_params& p, Hv
     if (p.B < 0 || p.Lq < 0 || p.Lk < 0 || p.heads <= 0 || p.kv_heads <= 0 || p.heads % p.kv_heads != 0) return -1;
     if (p.D != 40 && p.D != 64 && p.D != 80 && p.D != 128 && p.D != 160) return -2;
     const long rows = (long)p.Lq * (p.heads / p.kv_heads), pairs = (long)p.B * p.kv_heads;
-    if (rows > 0x3fffffffL || pairs > 0x3fffffffL) return -1;
+    if (rows > 0x3fffffffL || pairs > 0x3fffffffL || p.Lk > 0x3fffffff) return -1;
     a.p = p;
     a.G = p.heads / p.kv_heads;
     a.rows = (int)rows;
@@ -796,7 +796,7 @@ static inline int hv_cross_attention_plan(const hv_cross_attention_params& p, Hv
         a.run = (int)(all / 64 < 1 ? 1 : all / 64 < a.blocks ? all / 64 : a.blocks);  // at least 64 runs: 8 for each XCD
         units = all;
     }
-    if (units > 0x3fffffffL) return -1;
+    if (!hv_fits_launch(units + 8L * a.run, 256)) return -1;
     a.units = (int)units;
     return 0;
 }

@@ -559,7 +559,7 @@ static inline int hv_gemm_fp8_plan(const hv_gemm_fp8_params& p, HvGemmFp8Args& a
     if (tile == 16) {
         a.tiles_m = 1;
         a.tiles_n = (p.N + 15) / 16;
-        return 0;
+        return hv_fits_launch(a.tiles_n, 512) ? 0 : -1;
     }
     a.tiles_m = (p.M + tile - 1) / tile;
     a.tiles_n = (p.N + tile - 1) / tile;
@@ -569,6 +569,7 @@ static inline int hv_gemm_fp8_plan(const hv_gemm_fp8_params& p, HvGemmFp8Args& a
         a.per = (a.kb + a.splits - 1) / a.splits;
         a.splits = (a.kb + a.per - 1) / a.per;
     }
+    if (tile == 64 && !hv_fits_launch(tiles(64) * a.splits, 256)) return -1;
     return 0;
 }
 
@@ -730,7 +731,7 @@ static inline int hv_fp8_quantize_launch(const HvQuantArgs& in, int block_rows, 
     a.kb = (a.K + 127) / 128;
     if (block_rows == 1) {
         const long wgs = ((long)a.M * a.kb + 15) / 16;
-        if (wgs > 0x7fffffffL) return -1;
+        if (!hv_fits_launch(wgs, 256)) return -1;
         hv_note("hv_fp8_quantize_rows_kernel | M=%d K=%d", a.M, a.K);
         hv_launch(hv_fp8_quantize_rows_kernel, dim3((unsigned)wgs), dim3(256), stream, a);
     } else {

@@ -224,10 +224,12 @@ int hv_attention_fp8(const hv_attention_params* p, const float* kscale, const fl
  * O[b][i][h] = sum_j softmax_j(scale Q[b][i][h] . K[b][j][g]) V[b][j][g],  g = h / (heads / kv_heads), over the attended states:
  * j < kv_len[b] and key_mask[b][j] != 0.  A batch entry with no attended state gets zeros, whatever its queries hold; what memory
  * holds in the other states (NaN included) does not reach the output, and states at or behind kv_len are not read.  A query that holds
- * NaN or infinity spoils its own row only.  Values are row-major.  All frames of a clip that share their half's prompt are ONE batch entry (Lq = frames * tokens).  O may be Q, and overlap nothing else.  Any Lq, Lk >= 0; D in
- * {40, 64, 80, 128, 160}; pointers 16-byte aligned, strides >= 0 in multiples of 8 elements (the batch strides of K, V and the mask may be 0:
- * shared states; rows of K and V at most 2^24 elements apart).  The keys are cut into ranges that are joined by a second launch where the queries alone would not fill the
- * chip: hv_cross_attention_workspace() floats of scratch, not to be shared by calls that may run at the same time. */
+ * NaN or infinity spoils its own row only.  Values are row-major.  All frames of a clip that share their half's prompt are ONE batch
+ * entry (Lq = frames * tokens).  O may be Q, and overlap nothing else.  Any Lq, Lk >= 0 (Lk up to 2^30, and what less than 2^32 threads
+ * cover); D in {40, 64, 80, 128, 160}; pointers 16-byte aligned, strides >= 0 in multiples of 8 elements (the batch strides of K, V and
+ * the mask may be 0: shared states; rows of K and V at most 2^24 elements apart).  The keys are cut into ranges that are joined by a
+ * second launch where the queries alone would not fill the chip: hv_cross_attention_workspace() floats of scratch, not to be shared by
+ * calls that may run at the same time. */
 typedef struct hv_cross_attention_params {
     const uint16_t* Q; /* row i of entry b at Q + b * q_stride_b + i * ldq, head h at column h*D */
     long ldq, q_stride_b;
@@ -254,7 +256,9 @@ int hv_cross_attention_workspace(const hv_cross_attention_params* p, long* float
  * nearest e4m3, ties to even (exactly: the quotient is not rounded before).  A NaN stays one and sets no scale; a block with an
  * infinity is NaN as a whole.  scale element (row block i, column block j) at scale[i * scale_row + j * scale_k].
  * hv_gemm_fp8: Y[m][n] = bias[n] + residual[m][n] + sum_kb x_scale[m][kb] w_scale[n/128][kb] (X . W^T over block kb), fp32 sums,
- * rounded once.  K a multiple of 16 (the last block may be short), X, W, Q rows 16-byte aligned; any M, N >= 0. */
+ * rounded once.  K a multiple of 16 (the last block may be short), X, W, Q rows 16-byte aligned; any M, N >= 0 that one launch (less than
+ * 2^32 threads) covers: N up to 2^27 - 16 where M <= 64, up to 2^28 - 16 blocks of one row, 65535 x 128 rows in blocks of 128.
+ * hv_gemm_fp8_workspace() floats of scratch, not to be shared by calls that may run at the same time. */
 int hv_fp8_quantize(const uint16_t* X, long ldx, int M, int K, int block_rows, uint8_t* Q, long ldq, float* scale, long scale_row,
                     long scale_k, void* stream);
 typedef struct hv_gemm_fp8_params {
