@@ -135,3 +135,16 @@ def test_states_narrower_than_the_packed_weights():
                     eng.set_encoder_hidden_states(torch.randn(2, tokens, width, generator=g))
     finally:
         hvlib.current_stream = restore
+
+
+def test_frames_of_a_shard(engine):  # noqa: F811
+    """an executor that holds some of the frames computes the rows that one with all of them does"""
+    eng = engine[0]
+    g = torch.Generator().manual_seed(19)
+    mask = torch.rand(2, 9, generator=g) < 0.6
+    mask[:, 0] = True
+    eng.set_encoder_hidden_states(torch.randn(2, 9, 768, generator=g), mask)
+    h = torch.randn(2, 3 * ROWS, 320, generator=g).to(BF16)  # three frames
+    want = _attend(eng, h)
+    for f0, f1 in ((0, 2), (2, 3)):
+        assert torch.equal(_attend(eng, h[:, f0 * ROWS:f1 * ROWS]), want[:, f0 * ROWS:f1 * ROWS])

@@ -47,3 +47,38 @@ def test_sizes_past_one_launch_are_refused(cx):  # noqa: F811
     for rows, M in ((1, 1 << 28), (128, 65536 * 128)):
         assert _rc(cx, "hv_fp8_quantize", at, 16, M, 16, rows, at, 16, at, 1, 1, None) == A.HV_EINVAL
         assert b"2^32" in cx.lib.cdll.hv_last_error()
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("Lq,Lk,heads,kv_heads,D", ec.CROSS_KERNELS)
+def test_a_query_that_is_no_number_stays_in_its_row(cx, Lq, Lk, heads, kv_heads, D, masked):  # noqa: F811
+    ec.case_query_values(cx, Lq, Lk, heads, kv_heads, D, masked, seed=Lk + 1)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("Lq,Lk,heads,kv_heads,D", ec.CROSS_KERNELS)
+def test_attended_states_that_are_no_numbers(cx, Lq, Lk, heads, kv_heads, D, masked):  # noqa: F811
+    ec.case_state_values(cx, Lq, Lk, heads, kv_heads, D, masked, seed=Lk + 2)
+
+
+GEMMS = [(5, 40, 272), (33, 24, 144), (100, 133, 272), (70, 50, 2064)]
+
+
+@pytest.mark.parametrize("out", [ec.BF16, ec.F32])
+@pytest.mark.parametrize("M,N,K", GEMMS)
+def test_gemm_fp8_operands_that_are_no_numbers(cx, M, N, K, out):  # noqa: F811
+    ec.case_gemm_values(cx, M, N, K, out, seed=M)
+
+
+@pytest.mark.parametrize("out", [ec.BF16, ec.F32])
+@pytest.mark.parametrize("tile", [64, 128, 256])
+def test_gemm_fp8_tiles_operands_that_are_no_numbers(cx, tile, out):  # noqa: F811
+    cx.lib.call("hv_set_tuning", 16, tile)
+    try:
+        ec.case_gemm_values(cx, 270, 140, 144, out, seed=tile)
+    finally:
+        cx.lib.call("hv_set_tuning", 16, 0)
+
+
+def test_command_list_of_a_product_in_ranges(cx):  # noqa: F811
+    ec.case_ranges_command_list(cx, M=66, N=40, K=2048)

@@ -17,3 +17,31 @@ def test_empty_entries_are_zero_whatever_they_hold(cx, Lq, Lk, heads, kv_heads, 
 @pytest.mark.parametrize("Lq,Lk,heads,kv_heads,D", SIZES)
 def test_masks_that_leave_whole_stretches_out(cx, Lq, Lk, heads, kv_heads, D):  # noqa: F811
     ec.case_masked_stretches(cx, Lq, Lk, heads, kv_heads, D, seed=Lk)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("Lq,Lk,heads,kv_heads,D", SIZES)
+def test_a_query_that_is_no_number_stays_in_its_row(cx, Lq, Lk, heads, kv_heads, D, masked):  # noqa: F811
+    ec.case_query_values(cx, Lq, Lk, heads, kv_heads, D, masked, seed=Lk + 1)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("Lq,Lk,heads,kv_heads,D", SIZES)
+def test_attended_states_that_are_no_numbers(cx, Lq, Lk, heads, kv_heads, D, masked):  # noqa: F811
+    ec.case_state_values(cx, Lq, Lk, heads, kv_heads, D, masked, seed=Lk + 2)
+
+
+@pytest.mark.parametrize("out", [ec.BF16, ec.F32])
+@pytest.mark.parametrize("M,N,K", [(5, 40, 272), (33, 24, 144), (100, 133, 272), (70, 50, 2064), (4100, 2050, 400)])
+def test_gemm_fp8_operands_that_are_no_numbers(cx, M, N, K, out):  # noqa: F811
+    ec.case_gemm_values(cx, M, N, K, out, seed=M)
+
+
+@pytest.mark.parametrize("out", [ec.BF16, ec.F32])
+@pytest.mark.parametrize("tile", [64, 128, 256])
+def test_gemm_fp8_tiles_operands_that_are_no_numbers(cx, tile, out):  # noqa: F811
+    cx.lib.call("hv_set_tuning", 16, tile)
+    try:
+        ec.case_gemm_values(cx, 270, 140, 144, out, seed=tile)
+    finally:
+        cx.lib.call("hv_set_tuning", 16, 0)
