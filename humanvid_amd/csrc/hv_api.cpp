@@ -135,7 +135,7 @@ int hv_cross_attention(const hv_cross_attention_params* p, void* stream) {
     if (p->B > 0 && p->Lq > 0 && (!p->Q || !p->O || (p->Lk > 0 && (!p->K || !p->V)))) return hv_fail(HV_EINVAL, "hv_cross_attention: null operand");
     int rc = hvk_cross_attention(*p, (hipStream_t)stream);
     if (rc == -2) return hv_fail(HV_ENOTSUP, "hv_cross_attention: head dim must be 40, 64, 80, 128 or 160");
-    if (rc == -3) return hv_fail(HV_EINVAL, "hv_cross_attention: workspace smaller than hv_cross_attention_workspace() floats");
+    if (rc == -3) return hv_fail(HV_EINVAL, "hv_cross_attention: need a workspace of hv_cross_attention_workspace() floats, 16-byte aligned");
     if (rc != 0)
         return hv_fail(HV_EINVAL, "hv_cross_attention: need sizes >= 0, heads a multiple of kv_heads, a scale in (0, 1e30], 16-byte aligned pointers, "
                                   "strides >= 0 in multiples of 8 elements, rows of K and V at most 2^24 elements apart, at most 2^30 states, less than 2^32 threads");

@@ -82,3 +82,12 @@ def test_gemm_fp8_tiles_operands_that_are_no_numbers(cx, tile, out):  # noqa: F8
 
 def test_command_list_of_a_product_in_ranges(cx):  # noqa: F811
     ec.case_ranges_command_list(cx, M=66, N=40, K=2048)
+
+
+def test_scratch_that_is_not_aligned_is_named(cx):  # noqa: F811
+    import torch
+
+    q, k = torch.zeros(1, 2, 40, dtype=ec.BF16), torch.zeros(1, 2000, 40, dtype=ec.BF16)
+    n = ec.ops.cross_attention(cx.lib, cx.stream, q, k, k, q.clone(), heads=1, query_workspace=True)
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        ec.ops.cross_attention(cx.lib, cx.stream, q, k, k, q.clone(), heads=1, workspace=torch.zeros(n + 1)[1:])
