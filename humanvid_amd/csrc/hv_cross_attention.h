@@ -140,10 +140,12 @@ HV_DEV bf16x8 hv_bf16_ones() { return bf16x8{0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3
 // ---- few states (Lk <= 16 NT <= 96, D <= 80): a prompt.  The stream of queries is what counts -- q is read once, o written once.
 // A workgroup takes four neighbouring query heads (4 / G key heads) and streams tiles of TQ queries through two LDS slots: the next
 // tile is in flight by LDS-DMA while this one is computed, the results replace the queries in the slot and leave it.  Both ways a
-// row's four heads are one run of memory (320 - 640 bytes).  At 2 x 147456 queries, 77 states, D = 40 (378 MB) the copies
-// alone take 85 us, all of it 103; a head at a time 99 / 115; straight from memory into operand registers (16 lanes in 16 rows) - / 133.
+// row's four heads are one run of memory (320 - 640 bytes).  At 2 x 147456 queries, 77 states, D = 40 (378 MB) it takes 90 - 96 us; a head
+// at a time took 115, straight from memory into operand registers (16 lanes in 16 rows) 133.
 // All of K and V^T of its key head stay in a wave's REGISTERS as matrix operands.  No running maximum: a row's scores are all there.
-// The number of 16-key tiles is a template argument: branches around absent tiles cost more than a masked tile.
+// The number of 16-key tiles is a template argument: branches around absent tiles cost more than a masked tile.  2, 4, 5 and 6 tiles are
+// there: 1 and 3 would spare little beside the stream of queries (16 states as one tile or two: 83.4 against 83.8 us at D = 40,
+// 32.4 against 32.8 at D = 80; 33 states as three or four: 86.9 against 87.8 and 35.1 against 36.2).
 template <int D, int NT>
 __global__ __launch_bounds__(256, D == 40 ? 3 : 2) void hv_cross_attention_few_kernel(HvCrossArgs a) {
     using G = HvCrossGeom<D>;
@@ -786,7 +788,7 @@ static inline int hv_cross_attention_plan(const hv_cross_attention_params& p, Hv
         const long base = pairs * a.blocks;
         if (base > 0 && base < 512 && p.Lk >= 2 * least) {
             // too few workgroups to fill the chip: cut the keys, to twice as many workgroups where entries may be of different lengths
-            // (4 x 1536 queries, up to 4109 states, D = 80: ragged 80 us against 97, all full 114 against 104)
+            // (4 x 1536 queries, up to 4109 states, D = 80: ragged 71 us against 89, all full 102 against 94)
             const long want = ((p.kv_len ? 1024 : 512) + base - 1) / base, most = p.Lk / least;
             a.splits = (int)(want < most ? want : most);
             a.per = ((p.Lk + a.splits - 1) / a.splits + 127) / 128 * 128;

@@ -4,8 +4,9 @@
 //   y[m][n] = bias[n] + residual[m][n] + sum_kb xs[m][kb] ws[n / 128][kb] sum_{k in block kb} x8[m][k] w8[n][k]
 //
 // A block of 128 is exactly one v_mfma_f32_16x16x128_f8f6f4: every instruction starts from a zero accumulator and its four
-// results per lane are added to the fp32 sums with the block's factor xs ws -- 4 v_fma per 32-cycle MFMA, 16 cycles that the matrix pipe
-// does not hide.
+// results per lane are added to the fp32 sums with the block's factor xs ws -- 4 v_fma per 32-cycle MFMA, of which the matrix pipe hides a
+// part (two waves a SIMD, 32 MFMAs and 128 v_fma a block in the order below: 539 ns, the MFMAs alone 462, the v_fma alone 128;
+// profiles/operators_fp8_parts.txt).
 // The operands are taken as A = W (rows n), B = X (columns m): a lane then owns ONE row m of Y per 16-row tile, so xs is one
 // value per lane and tile, and the four W tiles of a 64-column block are read from LDS in an order that leaves the lane twice
 // 8 consecutive columns: 16-byte stores, the four lanes of a row 64 bytes in one.
@@ -96,7 +97,7 @@ struct HvGemmFp8Args {
 };
 
 // 16 bytes at any address of an element: rows of Y and the residual need not be aligned (129774 x 900 x 64: 77 us, 257 with single
-// elements; 63515 x 1107 x 864 to fp32: 196 against 301)
+// elements; 63515 x 1107 x 864 to fp32: 179 against 301)
 HV_DEV u32x4 hv_ld16_any(const void* p) {
     u32x4 v;
     __builtin_memcpy(&v, p, 16);
@@ -143,13 +144,15 @@ HV_DEV void hv_gemm_fp8_store(const HvGemmFp8Args& a, int m, int n, float* v) {
 // ds_read_b128 on 16 different quarters of the 64 banks.  The pieces behind K in the last block hold repeated values of the same row;
 // their X side is zeroed in LDS.
 // Workgroups are persistent: the first block of the next tile is on its way while the last one of this tile is computed and its
-// results are stored -- one workgroup fills a CU's registers and LDS, so nothing else would cover that (147456 x 960 x 320: 131 -> 124 us;
-// 18432 x 10240 x 1280: 309 -> 306).
-// What bounds it: per block and wave 32 MFMAs (1024 cycles) and 128 fused multiply-adds for the block's scales (4 cycles each, which the
-// matrix pipe does not hide); a 256 x 256 tile takes 2.2 - 2.5 us a block (1640 - 1690 TFLOP/s at K = 1280).  Short reductions: the stores
-// (283 MB of the 330 MB at 147456 x 960 x 320), of which a tile's first block covers its predecessor's: 20 us for a block of all tiles,
-// 50 - 60 us for the results whatever K is.  (The second block requested ahead of the stores too costs a barrier more and was slower: 138.)
-// A whole tile's residual is requested four row tiles at a time (18432 x 10240 x 1280: 407 -> 376 us, 147456 x 960 x 320: 191 -> 182).
+// results are stored -- one workgroup fills a CU's registers and LDS, so nothing else would cover that (147456 x 960 x 320: 124 us, 131 with
+// a workgroup a tile).
+// What bounds it, from builds that leave a part out (profiles/operators_fp8_parts.txt): 18432 x 10240 x 1280 takes 286 us (1690 TFLOP/s),
+// 224 without the stores, 241 without the scales' multiply-adds, 236 without the copies, 183 without stores and multiply-adds.  The stores
+// (377 MB) are the largest part that nothing covers.  Short reductions even more so: 147456 x 960 x 320 (283 MB of results) takes 121 us,
+// 67 without the stores, 108 without the multiply-adds, 91 without the copies.  (The second block requested ahead of the stores too
+// costs a barrier more and was slower: 138.)
+// A whole tile's residual is requested four row tiles at a time (18432 x 10240 x 1280: 364 us, 407 when each row tile waits for its own;
+// 147456 x 960 x 320: 181 and 191).
 template <int WM, int WN, int MT, bool WIDE>
 __global__ __launch_bounds__(64 * WM * WN, 2) void hv_gemm_fp8_kernel(HvGemmFp8Args a) {
     constexpr int BM = WM * MT * 16, BN = WN * 64, WAVES = WM * WN;
@@ -550,9 +553,9 @@ static inline int hv_gemm_fp8_plan(const hv_gemm_fp8_params& p, HvGemmFp8Args& a
     auto tiles = [&](int t) { return (long)((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
     if (tiles(64) > 0x3fffffffL) return -1;
     const int want = g_hv_gemm_fp8_tile;
-    // 256 tiles take 3.5 times a 128 tile's CU time and run one to a CU in whole rounds, 128 tiles two to a CU (K = 2560, 36864 x 640: 95 against
-    // 78 us; 4096 x 4096 x 4096: 72 against 81); below 128 of the latter the 64 tiles' deeper pipeline and ranges are faster
-    // (1024 x 1280 x 5120: 28 against 38 us, 2048 x 1280 x 1280: 17.6 against 14.2).  An fp32 output's operands leave no room for 256.
+    // 256 tiles take 3.5 times a 128 tile's CU time and run one to a CU in whole rounds, 128 tiles two to a CU (K = 2560, 36864 x 640: 86 against
+    // 73 us; 4096 x 4096 x 4096: 66 against 74); below 128 of the latter the 64 tiles' deeper pipeline and ranges are faster
+    // (80 of them, 1024 x 1280 x 5120: 27 us, with 128 tiles 38; 160, 2048 x 1280 x 1280: 16 against 13).  An fp32 output's operands leave no room for 256.
     const long t256 = tiles(256), t128 = tiles(128);
     const bool large = !p.out_f32 && (t256 + 255) / 256 * 7 < 2 * (t128 < 512 ? 2 : (t128 + 255) / 256);
     tile = p.M <= 64 ? 16 : want ? (want == 256 && p.out_f32 ? 128 : want) : large ? 256 : t128 >= 128 ? 128 : 64;

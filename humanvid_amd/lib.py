@@ -48,7 +48,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def current_stream() -> int:
-    """the handle of torch's current stream on the current device (read without making a Stream object: 2.8 -> 0.4 us a call)"""
+    """the handle of torch's current stream on the current device (read without making a Stream object: 2.7 -> 0.24 us a call)"""
     if _raw_stream is None:
         return torch.cuda.current_stream().cuda_stream
     return _raw_stream(torch.cuda.current_device())
