@@ -496,6 +496,14 @@ HV_DEV void hv_gemm_epilogue_fast_perm(const HvGemmParams& p, f32x4 (&acc)[4][NM
                 }
                 outp[mf][h] = o;
             }
+#ifndef HV_EMU
+            if (STATS == 1) {  // added up here: hipcc would move all the sums behind the stores and keep every fragment's values for them
+#pragma unroll
+                for (int nf = 0; nf < 4; ++nf)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(gs[nf][e]), "+v"(gq[nf][e]));
+            }
+#endif
         }
 #if !defined(HV_EMU)
         __builtin_amdgcn_sched_barrier(0);  // ... and the next group's loads are not hoisted over it (register budget)
