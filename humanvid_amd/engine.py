@@ -258,6 +258,19 @@ class UNet3DEngine:
                 self.cross_const[loc] = c
             ops.gemm(self.lib, st, v, self.w[t + ".attn2.to_out.0.w"], c, bias=self.w[t + ".attn2.to_out.0.bias"])
 
+    def _check_states(self, B: int):
+        """the encoder states cover the batch: a row of the folded constants, or keys | values, for every entry"""
+        table = self.cross_kv or self.cross_const
+        if not table:
+            return
+        have = next(iter(table.values())).shape[0]
+        if self.cfg_half is not None and B == 1:
+            ok = have > self.cfg_half
+        else:  # (a batch of one reads the first row of the folded constants)
+            ok = have == B if self.cross_kv else have >= B
+        if not ok:
+            raise ValueError(f"encoder_hidden_states: {have} batch entries for a batch of {B}")
+
     def _packed_states(self, ehs: torch.Tensor) -> torch.Tensor:
         """[B, L, channels] -> [B * L, channels up to a multiple of 64, as the packed weights have], bf16 on the device, zeros behind"""
         e = self._dev(ehs.reshape(-1, ehs.shape[2]), BF16)
@@ -431,6 +444,7 @@ class UNet3DEngine:
         L, st, w, ws = self.lib, self.stream, self.w, self.ws
         n, H, W, _ = x_in.shape
         assert n == B * F
+        self._check_states(B)
         boc = tuple(self.cfg["block_out_channels"])
         G = self.groups
 

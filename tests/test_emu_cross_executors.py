@@ -148,3 +148,28 @@ def test_frames_of_a_shard(engine):  # noqa: F811
     want = _attend(eng, h)
     for f0, f1 in ((0, 2), (2, 3)):
         assert torch.equal(_attend(eng, h[:, f0 * ROWS:f1 * ROWS]), want[:, f0 * ROWS:f1 * ROWS])
+
+
+@pytest.mark.parametrize("tokens", [1, 4])
+def test_states_of_too_few_entries_are_refused_before_anything_runs(engine, tokens, monkeypatch):  # noqa: F811
+    """a forward of two batch entries with the states of one: the second entry's row lies behind the table"""
+    from humanvid_amd import engine as E
+
+    eng = engine[0]
+
+    def launched(*a, **kw):
+        raise AssertionError("a kernel was launched")
+
+    def forward(e, B):
+        return e.forward_nhwc(torch.zeros(2 * B, 8, 4, 32, dtype=BF16), torch.zeros(B), None, B=B, F=2)
+
+    halves = [_half(eng, i) for i in (0, 1)]
+    eng.cross_const.clear()  # (a table of this test's own: one row)
+    eng.set_encoder_hidden_states(torch.randn(1, tokens, 768))
+    monkeypatch.setattr(E.ops, "timestep_embedding", launched)  # the first kernel of a forward
+    for e, B in ((eng, 2), (halves[1], 1)):
+        with pytest.raises(ValueError, match="batch entries"):
+            forward(e, B)
+    for e in (eng, halves[0]):  # one entry: as far as the first kernel
+        with pytest.raises(AssertionError, match="launched"):
+            forward(e, 1)
